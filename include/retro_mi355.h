@@ -13,7 +13,8 @@
  *  - Element type of K/V/centroid/query data is bfloat16 (uint16 bit patterns); every entry point whose
  *    arithmetic depends on the element type has a twin with the suffix _f16 for IEEE half (the copy and
  *    permutation entry points move 16-bit elements of either type).
- *    head_dim must be 128 (the reference hard-codes it: gather_copy.cu:196-199).
+ *    head_dim must be 128 (the reference hard-codes it: gather_copy.cu:196-199); the paged cache takes 64 as well and has
+ *    the element type in its struct.
  *  - Return value: RI_OK (0) or a negative RI_ERR_* code; ri_status_string() names it
  *    and ri_last_hip_error() returns the HIP error behind RI_ERR_LAUNCH.
  *  - "group" g = batch * kv_heads + kv_head, BG groups in total; gs = query heads per
@@ -659,6 +660,77 @@ int ri_prefill_index(const void* centroids, const void* mean, const int32_t* cou
 int ri_prefill_index_f16(const void* centroids, const void* mean, const int32_t* counts, const int32_t* offsets,
                          void* out, uint8_t* mask, void* size16, int32_t* size, int32_t* start, int H, int nc,
                          ri_stream_t stream);
+
+/* ------------------------------------------------------------------------------------
+ * Paged key-value cache: attention of a new token, append, write of a prompt, eviction by accumulated attention weight.
+ * No counterpart in the reference.
+ * ---------------------------------------------------------------------------------- */
+
+/* A layer's pages (host memory, read during the call).  Page p of head h holds page_rows rows of `dim` elements from
+ * k_pages + p * k_page_stride + h * k_head_stride on, k_row_stride apart (elements; multiples of 8, the base 16-byte aligned), and so
+ * do the values.  Row r of sequence b is row r % page_rows of page block_table[b * table_stride + r / page_rows]; an entry outside
+ * [0, pages) is a page that is not there: its rows are neither attended nor written.  dim 64 or 128, page_rows a power of two, at
+ * most 2^24 rows to a sequence.  half: IEEE half instead of bfloat16. */
+typedef struct ri_paged_t {
+  void* k_pages;
+  void* v_pages;
+  const int32_t* block_table;
+  int64_t k_page_stride, k_head_stride, k_row_stride;
+  int64_t v_page_stride, v_head_stride, v_row_stride;
+  int64_t table_stride;
+  int pages, heads, page_rows, dim, table_pages, half;
+} ri_paged_t;
+
+/* Attention of one token of each of B sequences over its rows [starts[b], lens[b]) (starts NULL: from 0 on; both clamped to
+ * [0, max_len], max_len at most the rows of the block table): out[b, i, :] = sum_r p_r v_r with p = softmax(scale q[b, i, :].k_r),
+ * q and out [B, heads * gs, dim] contiguous, gs <= 16; lse_out [B, heads * gs] fp32 (or NULL) the log of the sum of the
+ * exponentials.  No rows: zeros and -inf.  With scores, the weights p_r summed over the gs heads of head h are added to
+ * scores[b * score_batch_stride + h * score_head_stride + r] (fp32, score_head_stride >= max_len).  The workspace needs no
+ * initialisation; calls that may overlap must not share it. */
+size_t ri_paged_attention_workspace_bytes(int B, int heads, int gs, int dim, int max_len, int scored);
+int ri_paged_attention(const ri_paged_t* cache, const void* q, const int32_t* lens, const int32_t* starts, float* scores,
+                       int64_t score_batch_stride, int64_t score_head_stride, void* out, float* lse_out, int B, int gs,
+                       int max_len, float scale, void* workspace, size_t workspace_bytes, ri_stream_t stream);
+
+/* Appends a token's key and value of each head, at key + b * key_batch_stride + h * key_head_stride, to each of B sequences.  A
+ * sequence of n = lens[b] < budget rows takes them as row n.  Of a full one, with scores, they take the place of the row with the
+ * lowest score in each head (equal scores: the lowest row; NaN counts as the highest), of those whose token is neither one of the
+ * first `sinks` nor one of the last `recent`, the new one among them (if none is left, row 0); without scores nothing is written.
+ * new_lens[b] = min(n + 1, budget) (another buffer than lens; may be NULL).  The row's score becomes 0 and its position, where
+ * positions are given, token_positions[b], the token's place in the sequence.  sinks + recent < budget <= rows of the block table. */
+int ri_paged_append(const ri_paged_t* cache, const void* key, const void* value, int64_t key_batch_stride,
+                    int64_t key_head_stride, int64_t value_batch_stride, int64_t value_head_stride, const int32_t* lens,
+                    int32_t* new_lens, float* scores, int64_t score_batch_stride, int64_t score_head_stride,
+                    int32_t* positions, int64_t position_batch_stride, int64_t position_head_stride,
+                    const int32_t* token_positions, int B, int budget, int sinks, int recent, ri_stream_t stream);
+
+/* Writes the prompts of B sequences, seqlens[b] (NULL: T) of T tokens each, into their pages from row 0 on.  Of a prompt of more
+ * than `budget` tokens, each head keeps `budget`: the first `sinks`, the last `recent` and of the others those with the highest
+ * weights[b, h, :] (order as above, equal weights: the first ones), in their order.  new_lens[b] = rows written (may be NULL);
+ * scores and positions of the rows, where given, become the kept weights and the tokens' places.  weights may be NULL if T <=
+ * budget and scores is.  sinks + recent <= budget. */
+size_t ri_paged_fill_workspace_bytes(int B, int heads, int T, int budget);
+int ri_paged_fill(const ri_paged_t* cache, const void* key, const void* value, int64_t key_batch_stride,
+                  int64_t key_token_stride, int64_t key_head_stride, int64_t value_batch_stride, int64_t value_token_stride,
+                  int64_t value_head_stride, const int32_t* seqlens, const float* weights, int64_t weight_batch_stride,
+                  int64_t weight_head_stride, int32_t* new_lens, float* scores, int64_t score_batch_stride,
+                  int64_t score_head_stride, int32_t* positions, int64_t position_batch_stride,
+                  int64_t position_head_stride, int B, int T, int budget, int sinks, int recent, void* workspace,
+                  size_t workspace_bytes, ri_stream_t stream);
+
+/* out[b, h, j] (fp32, [B, heads, T]) = sum over the gs query heads of head h and over the W queries of sequence b of the causal
+ * attention weight that key j gets: query i is that of token seqlens[b] - W + i (seqlens NULL: T) and sees the keys up to its own;
+ * queries of tokens before 0 weigh nothing, keys from seqlens[b] on get 0.  q [B, W, heads * gs, dim] and key [B, T, heads, dim]
+ * with strides in elements, multiples of 8; W <= T, gs <= 16, dim 64 or 128.  The workspace needs no initialisation. */
+size_t ri_attention_weights_workspace_bytes(int B, int heads, int gs, int W, int T);
+int ri_attention_weights(const void* q, const void* key, const int32_t* seqlens, float* out, int64_t q_batch_stride,
+                         int64_t q_token_stride, int64_t q_head_stride, int64_t key_batch_stride, int64_t key_token_stride,
+                         int64_t key_head_stride, int B, int W, int T, int heads, int gs, int dim, float scale,
+                         void* workspace, size_t workspace_bytes, ri_stream_t stream);
+int ri_attention_weights_f16(const void* q, const void* key, const int32_t* seqlens, float* out, int64_t q_batch_stride,
+                             int64_t q_token_stride, int64_t q_head_stride, int64_t key_batch_stride,
+                             int64_t key_token_stride, int64_t key_head_stride, int B, int W, int T, int heads, int gs,
+                             int dim, float scale, void* workspace, size_t workspace_bytes, ri_stream_t stream);
 
 /* ------------------------------------------------------------------------------------
  * Host wave buffer (LRU block cache manager + K/V re-organisation) and its thread pool

@@ -32,6 +32,13 @@ class Lru(C.Structure):
             "buffer_size", "capacity", "block", "BG")]
 
 
+class Paged(C.Structure):
+    """ri_paged_t"""
+    _fields_ = [(n, P) for n in ("k_pages", "v_pages", "block_table")] + [(n, I64) for n in (
+        "k_page_stride", "k_head_stride", "k_row_stride", "v_page_stride", "v_head_stride", "v_row_stride",
+        "table_stride")] + [(n, I) for n in ("pages", "heads", "page_rows", "dim", "table_pages", "half")]
+
+
 # name -> (restype, argtypes); mirrors include/retro_mi355.h
 SIGNATURES = {
     "ri_status_string": (C.c_char_p, [I]),
@@ -107,6 +114,14 @@ SIGNATURES = {
     "ri_prefill_center_f16": (I, [P, P, I, I, P]),
     "ri_prefill_index": (I, [P] * 9 + [I, I, P]),
     "ri_prefill_index_f16": (I, [P] * 9 + [I, I, P]),
+    "ri_paged_attention_workspace_bytes": (SZ, [I] * 6),
+    "ri_paged_attention": (I, [P] * 5 + [I64, I64, P, P, I, I, I, F, P, SZ, P]),
+    "ri_paged_append": (I, [P] * 3 + [I64] * 4 + [P] * 3 + [I64, I64, P, I64, I64, P, I, I, I, I, P]),
+    "ri_paged_fill_workspace_bytes": (SZ, [I] * 4),
+    "ri_paged_fill": (I, [P] * 3 + [I64] * 6 + [P, P, I64, I64, P, P, I64, I64, P, I64, I64] + [I] * 5 + [P, SZ, P]),
+    "ri_attention_weights_workspace_bytes": (SZ, [I] * 5),
+    "ri_attention_weights": (I, [P] * 4 + [I64] * 6 + [I] * 6 + [F, P, SZ, P]),
+    "ri_attention_weights_f16": (I, [P] * 4 + [I64] * 6 + [I] * 6 + [F, P, SZ, P]),
     "ri_threadpool_create": (P, [I]),
     "ri_threadpool_create_pinned": (P, [I, I]),
     "ri_threadpool_pinned_workers": (I, [P]),

@@ -14,7 +14,7 @@ import weakref
 
 import torch
 
-from ._lib import DecodeStep, Lru, lib, check, step_calls
+from ._lib import DecodeStep, Lru, Paged, lib, check, step_calls
 
 # 16-bit element types of the reference's operators and cache (batch_gemm_softmax.cu:185-197,
 # gather_copy.cu:63-67): every wrapper takes either and calls the entry point of that type (name or name_f16).
@@ -806,3 +806,228 @@ def prefill_index(centroids, mean, counts, offsets, out, mask, size16, size, sta
 def permute_rows(src, members, dst, P, N, in_stride_rows, out_stride_rows):
     check(lib().ri_permute_rows(_p(src), _p(members), _p(dst), P, N, in_stride_rows, out_stride_rows, _stream()),
           "permute_rows")
+
+
+# ----------------------------------------------------------------------------------------
+# paged key-value cache
+# ----------------------------------------------------------------------------------------
+PAGED_DIMS = (64, 128)
+
+
+def _on(device):
+    """The context in which launches and `_stream` belong to `device`."""
+    return contextlib.nullcontext() if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
+
+
+def _strided(t, dims, dtype, device, name, writes=False):
+    """Strides of all but the last dimension of a tensor whose rows are read or written 16 bytes at a time (of dimensions of one
+    element: 0)."""
+    if not isinstance(t, torch.Tensor) or t.dim() != dims:
+        raise ValueError(f"{name}: expected a tensor of {dims} dimensions")
+    if t.dtype != dtype:
+        raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
+    if t.device != device:
+        raise ValueError(f"{name}: expected a tensor on {device}")
+    strides = [st if n > 1 else 0 for n, st in zip(t.shape[:-1], t.stride()[:-1])]
+    if t.stride(-1) != 1 or any(st % 8 for st in strides) or t.data_ptr() % 16:
+        raise ValueError(f"{name}: rows must be contiguous and 16-byte aligned")
+    if writes and any(st == 0 for n, st in zip(t.shape[:-1], strides) if n > 1):
+        raise ValueError(f"{name}: written, and its elements share memory")
+    return strides
+
+
+def _table32(t, shape, device, name):
+    """A device tensor of int32 of this shape (None: any size), rows contiguous; its row stride."""
+    if not isinstance(t, torch.Tensor) or t.dim() != len(shape) or any(n is not None and m != n for m, n in zip(t.shape, shape)):
+        raise ValueError(f"{name}: expected a tensor of shape {tuple('any' if n is None else n for n in shape)}")
+    if t.dtype != torch.int32:
+        raise TypeError(f"{name}: expected torch.int32, got {t.dtype}")
+    if t.device != device:
+        raise ValueError(f"{name}: expected a tensor on {device}")
+    if t.numel() and t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{name}: expected contiguous rows")
+    return t.stride(0)
+
+
+def _per_row(t, dtype, B, heads, rows, device, name, writes=True):
+    """Strides (sequence, head) of a tensor [B, heads, rows or more] with a value to each row; (0, 0) for None."""
+    if t is None:
+        return 0, 0
+    if not isinstance(t, torch.Tensor) or t.dim() != 3 or t.shape[0] != B or t.shape[1] != heads or t.shape[2] < rows:
+        raise ValueError(f"{name}: expected [{B}, {heads}, {rows} or more]")
+    if t.dtype != dtype:
+        raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
+    if t.device != device:
+        raise ValueError(f"{name}: expected a tensor on {device}")
+    if t.shape[2] > 1 and t.stride(2) != 1:
+        raise ValueError(f"{name}: expected contiguous rows")
+    sb, sh = (t.stride(0) if B > 1 else 0), (t.stride(1) if heads > 1 else t.shape[2])
+    if sh < rows or (B > 1 and sb < rows) or (writes and B > 1 and heads > 1 and
+                                              not (sb >= (heads - 1) * sh + rows or sh >= (B - 1) * sb + rows)):
+        raise ValueError(f"{name}: its elements share memory")
+    return sb, sh
+
+
+def _paged(k_pages, v_pages, block_table, B, writes=False):
+    """ri_paged_t of the pages [pages, heads, page_rows, dim] and of the block table [B, n]."""
+    if not isinstance(k_pages, torch.Tensor) or not k_pages.is_cuda:
+        raise ValueError("k_pages: expected a device tensor")
+    if k_pages.dtype not in _DT:
+        raise RuntimeError("Only Half and BFloat16 are supported")
+    device = k_pages.device
+    ks = _strided(k_pages, 4, k_pages.dtype, device, "k_pages", writes)
+    vs = _strided(v_pages, 4, k_pages.dtype, device, "v_pages", writes)
+    pages, heads, rows, dim = k_pages.shape
+    if v_pages.shape != k_pages.shape:
+        raise ValueError("k_pages and v_pages: expected the same shape")
+    if dim not in PAGED_DIMS or rows < 1 or rows & (rows - 1) or pages < 1 or heads < 1:
+        raise ValueError("k_pages: expected [pages, heads, a power of two, 64 or 128]")
+    ts = _table32(block_table, (B, None), device, "block_table")
+    n = block_table.shape[1]
+    if n < 1 or n * rows > 1 << 24:
+        raise ValueError("block_table: expected 1 to 2^24 rows to a sequence")
+    return Paged(k_pages=_p(k_pages), v_pages=_p(v_pages), block_table=_p(block_table), k_page_stride=ks[0], k_head_stride=ks[1],
+                 k_row_stride=ks[2], v_page_stride=vs[0], v_head_stride=vs[1], v_row_stride=vs[2], table_stride=ts, pages=pages,
+                 heads=heads, page_rows=rows, dim=dim, table_pages=n, half=int(k_pages.dtype == torch.float16))
+
+
+@_ranged("paged_attention")
+def paged_attention(q, k_pages, v_pages, block_table, cache_seqlens, starts=None, scores=None, scale=None,
+                    return_softmax_lse=False, max_len=None, scratch=None):
+    """Attention of one new token of each sequence over the rows of its pages (the token's own appended before).
+    q [B, 1, heads * gs, dim]; k_pages, v_pages [pages, heads, page_rows, dim] (strided or not, page_rows a power of two, dim 64 or
+    128); block_table [B, n] int32, the pages of a sequence in order; cache_seqlens [B] int32, the rows in use.  An entry of the
+    table that is no page of the pool stands for rows that are not there.  starts [B] int32: the first row that is attended.
+    scores [B, heads, rows] fp32: each row's weights, summed over the gs query heads of its head, are added to it.
+    max_len: no sequence has more rows (default: what the table holds; rows from max_len on are not attended), which sizes the
+    split over workgroups and the workspace.  Returns out like q, zeros where no row is attended, and with return_softmax_lse the
+    log-sum-exp [B, heads * gs] (-inf there).  `scratch`: the caller's own Scratch, where calls may overlap others."""
+    if not isinstance(q, torch.Tensor) or q.dim() != 4 or q.shape[1] != 1 or q.shape[0] < 1:
+        raise ValueError("paged_attention: expected q [B, 1, heads, dim]")
+    B, _, hq, dim = q.shape
+    cache = _paged(k_pages, v_pages, block_table, B)
+    _need(q, k_pages.dtype, "q")
+    if q.device != k_pages.device or q.data_ptr() % 16:
+        raise ValueError(f"q: expected a 16-byte aligned tensor on {k_pages.device}")
+    gs = hq // cache.heads
+    if dim != cache.dim or hq != gs * cache.heads or not 1 <= gs <= MAX_GROUP_SIZE:
+        raise ValueError("paged_attention: expected 1 to 16 query heads of the pages' dim to each of their heads")
+    room = cache.table_pages * cache.page_rows
+    max_len = room if max_len is None else int(max_len)
+    if not 1 <= max_len <= room:
+        raise ValueError(f"max_len: expected 1 to {room}, the rows that the block table holds")
+    _table32(cache_seqlens, (B,), q.device, "cache_seqlens")
+    if starts is not None:
+        _table32(starts, (B,), q.device, "starts")
+    sb, sh = _per_row(scores, torch.float32, B, cache.heads, max_len, q.device, "scores")
+    with _on(q.device):
+        out = torch.empty_like(q)
+        lse = torch.empty((B, hq), dtype=torch.float32, device=q.device) if return_softmax_lse else None
+        nbytes = lib().ri_paged_attention_workspace_bytes(B, cache.heads, gs, dim, max_len, int(scores is not None))
+        ws = _workspace(nbytes, q.device, "paged", scratch)
+        check(lib().ri_paged_attention(ctypes.byref(cache), _p(q), _p(cache_seqlens), _p(starts), _p(scores), sb, sh, _p(out),
+                                       _p(lse), B, gs, max_len, 1.0 / math.sqrt(dim) if scale is None else float(scale), _p(ws),
+                                       ws.numel(), _stream()), "paged_attention")
+    return (out, lse) if return_softmax_lse else out
+
+
+def paged_append(key, value, k_pages, v_pages, block_table, cache_seqlens, new_seqlens=None, scores=None, positions=None,
+                 token_positions=None, budget=None, sinks=0, recent=0):
+    """Writes a token's key and value [B, 1, heads, dim] into the pages.  A sequence with fewer than `budget` rows (default: what
+    the table holds) takes them as its next row; in a full one, given `scores` [B, heads, rows] fp32, `positions` [B, heads, rows]
+    int32 and `token_positions` [B] int32 (the token's place in its sequence), they take the place of the row with the lowest score
+    in each head, the first `sinks` and the last `recent` tokens of the sequence (the new one is the last) excepted; equal scores:
+    the lowest row.  The row's score becomes 0, its position the token's.  A full sequence without scores is left as it is.
+    new_seqlens [B] int32, another tensor than cache_seqlens: the rows in use afterwards."""
+    if not isinstance(key, torch.Tensor) or key.dim() != 4 or key.shape[1] != 1 or key.shape[0] < 1:
+        raise ValueError("paged_append: expected key [B, 1, heads, dim]")
+    B = key.shape[0]
+    cache = _paged(k_pages, v_pages, block_table, B, writes=True)
+    device, dtype = k_pages.device, k_pages.dtype
+    if key.shape[2:] != (cache.heads, cache.dim) or getattr(value, "shape", None) != key.shape:
+        raise ValueError("paged_append: expected key and value of the pages' heads and dim")
+    ks, vs = _strided(key, 4, dtype, device, "key"), _strided(value, 4, dtype, device, "value")
+    room = cache.table_pages * cache.page_rows
+    budget = room if budget is None else int(budget)
+    if not 1 <= budget <= room or sinks < 0 or recent < 0 or sinks + recent >= budget:
+        raise ValueError(f"budget: expected 1 to {room}, the rows that the block table holds, and more than sinks + recent")
+    _table32(cache_seqlens, (B,), device, "cache_seqlens")
+    if new_seqlens is not None:
+        _table32(new_seqlens, (B,), device, "new_seqlens")
+        if new_seqlens.data_ptr() == cache_seqlens.data_ptr():
+            raise ValueError("new_seqlens: expected another tensor than cache_seqlens")
+    if (scores is not None and positions is None) or (positions is not None and token_positions is None):
+        raise ValueError("paged_append: scores go with positions, and those with token_positions")
+    if token_positions is not None:
+        _table32(token_positions, (B,), device, "token_positions")
+    sb, sh = _per_row(scores, torch.float32, B, cache.heads, budget, device, "scores")
+    pb, ph = _per_row(positions, torch.int32, B, cache.heads, budget, device, "positions")
+    with _on(device):
+        check(lib().ri_paged_append(ctypes.byref(cache), _p(key), _p(value), ks[0], ks[2], vs[0], vs[2], _p(cache_seqlens),
+                                    _p(new_seqlens), _p(scores), sb, sh, _p(positions), pb, ph, _p(token_positions), B, budget,
+                                    sinks, recent, _stream()), "paged_append")
+
+
+def paged_fill(key, value, k_pages, v_pages, block_table, new_seqlens=None, seqlens=None, weights=None, scores=None,
+               positions=None, budget=None, sinks=0, recent=0, scratch=None):
+    """Writes prompts, key and value [B, T, heads, dim], into the pages from row 0 on; seqlens [B] int32: their lengths (default
+    T).  Of a prompt of more than `budget` tokens (default: the rows that the table holds) each head keeps `budget`: the first
+    `sinks`, the last `recent` and of the others those with the highest weights [B, heads, T] fp32 (attention_weights), at equal
+    weights the first ones, in their order.  new_seqlens [B] int32: the rows written.  scores, positions [B, heads, rows]: take the
+    kept weights and the tokens' places."""
+    if not isinstance(key, torch.Tensor) or key.dim() != 4 or key.shape[0] < 1 or key.shape[1] < 1:
+        raise ValueError("paged_fill: expected key [B, T, heads, dim]")
+    B, T = key.shape[:2]
+    cache = _paged(k_pages, v_pages, block_table, B, writes=True)
+    device, dtype = k_pages.device, k_pages.dtype
+    if key.shape[2:] != (cache.heads, cache.dim) or getattr(value, "shape", None) != key.shape:
+        raise ValueError("paged_fill: expected key and value of the pages' heads and dim")
+    ks, vs = _strided(key, 4, dtype, device, "key"), _strided(value, 4, dtype, device, "value")
+    room = cache.table_pages * cache.page_rows
+    budget = room if budget is None else int(budget)
+    if not 1 <= budget <= room or sinks < 0 or recent < 0 or sinks + recent > budget:
+        raise ValueError(f"budget: expected 1 to {room}, the rows that the block table holds, and at least sinks + recent")
+    if T > 1 << 24 or weights is None and (T > budget or scores is not None):
+        raise ValueError("paged_fill: weights tell which rows of a prompt beyond the budget are kept, and the rows' scores")
+    for t, nm in ((seqlens, "seqlens"), (new_seqlens, "new_seqlens")):
+        if t is not None:
+            _table32(t, (B,), device, nm)
+    if seqlens is not None and new_seqlens is not None and seqlens.data_ptr() == new_seqlens.data_ptr():
+        raise ValueError("new_seqlens: expected another tensor than seqlens")
+    wb, wh = _per_row(weights, torch.float32, B, cache.heads, T, device, "weights", writes=False)
+    sb, sh = _per_row(scores, torch.float32, B, cache.heads, min(T, budget), device, "scores")
+    pb, ph = _per_row(positions, torch.int32, B, cache.heads, min(T, budget), device, "positions")
+    with _on(device):
+        nbytes = lib().ri_paged_fill_workspace_bytes(B, cache.heads, T, budget)
+        ws = _workspace(nbytes, device, "paged_fill", scratch) if nbytes else None
+        check(lib().ri_paged_fill(ctypes.byref(cache), _p(key), _p(value), *ks, *vs, _p(seqlens), _p(weights), wb, wh,
+                                  _p(new_seqlens), _p(scores), sb, sh, _p(positions), pb, ph, B, T, budget, sinks, recent, _p(ws),
+                                  nbytes, _stream()), "paged_fill")
+
+
+@_ranged("attention_weights")
+def attention_weights(q, key, seqlens=None, scale=None, scratch=None):
+    """The causal attention weights that the last W tokens of each prompt give its keys, summed over them and over the gs query
+    heads of a key-value head: fp32 [B, heads, T], 0 past a prompt's end.  q [B, W, heads * gs, dim], the queries of the last W
+    tokens (of all: W = T); key [B, T, heads, dim]; seqlens [B] int32: the prompts' lengths (default T), query i being that of token
+    seqlens[b] - W + i (one before token 0 weighs nothing)."""
+    if not isinstance(q, torch.Tensor) or not isinstance(key, torch.Tensor) or q.dim() != 4 or key.dim() != 4 or not key.is_cuda:
+        raise ValueError("attention_weights: expected device tensors q [B, W, heads * gs, dim] and key [B, T, heads, dim]")
+    if key.dtype not in _DT:
+        raise RuntimeError("Only Half and BFloat16 are supported")
+    B, W, hq, dim = q.shape
+    T, heads = key.shape[1:3]
+    if key.shape[0] != B or key.shape[3] != dim or dim not in PAGED_DIMS or not 1 <= W <= T <= 1 << 24 or B < 1 or heads < 1 or \
+            hq % heads or not 1 <= hq // heads <= MAX_GROUP_SIZE or B * heads > 65535:
+        raise ValueError("attention_weights: expected q [B, W <= T, heads * 1 .. 16, dim] and key [B, T, heads, 64 or 128]")
+    qs, ks = _strided(q, 4, key.dtype, key.device, "q"), _strided(key, 4, key.dtype, key.device, "key")
+    if seqlens is not None:
+        _table32(seqlens, (B,), key.device, "seqlens")
+    with _on(key.device):
+        out = torch.empty((B, heads, T), dtype=torch.float32, device=key.device)
+        nbytes = lib().ri_attention_weights_workspace_bytes(B, heads, hq // heads, W, T)
+        ws = _workspace(nbytes, key.device, "weights", scratch)
+        check(_fn("ri_attention_weights", key.dtype)(
+            _p(q), _p(key), _p(seqlens), _p(out), *qs, *ks, B, W, T, heads, hq // heads, dim,
+            1.0 / math.sqrt(dim) if scale is None else float(scale), _p(ws), ws.numel(), _stream()), "attention_weights")
+    return out

@@ -1,0 +1,315 @@
+"""The paged cache's operators against their definition in 64 bits (oracle/paged.py), at the sizes and masks where they can go
+wrong.  Tolerances count roundings: u = eps / 2 of the element type is a rounding's largest relative error, 2^-24 that of fp32."""
+import math
+
+import pytest
+import torch
+
+from oracle import paged as oracle
+from retrievalattention_amd import kernels
+
+pytestmark = pytest.mark.gpu
+
+BF, HF = torch.bfloat16, torch.float16
+F = 2.0 ** -24
+
+
+def _u(dt):
+    return torch.finfo(dt).eps / 2
+
+
+def _randn(gen, *shape):
+    return torch.randn(*shape, generator=gen)
+
+
+def _pool(gen, dt, B, heads, dim, page, rows, junk=True):
+    """Pages of B sequences, scattered, with NaN and infinities in the rows behind each sequence's `rows` and in a spare page."""
+    per = -(-rows // page)
+    pool = B * per + 2
+    table = torch.randperm(pool - 1, generator=gen)[:B * per].view(B, per).to(torch.int32)
+    k, v = _randn(gen, pool, heads, page, dim).to(dt), _randn(gen, pool, heads, page, dim).to(dt)
+    if junk:
+        k[pool - 1], v[pool - 1] = math.nan, math.inf
+    return k, v, table
+
+
+def _spoil(k, v, table, lens, starts=None):
+    """Rows that are not attended hold NaN and infinities."""
+    page = k.shape[2]
+    for b in range(table.shape[0]):
+        for r in range(table.shape[1] * page):
+            if r >= int(lens[b]) or (starts is not None and r < int(starts[b])):
+                p = int(table[b, r // page])
+                if 0 <= p < k.shape[0]:
+                    k[p, :, r % page] = math.nan if r % 2 else math.inf
+                    v[p, :, r % page] = -math.inf if r % 3 else math.nan
+
+
+def _check_attention(q, k, v, table, lens, starts, out, lse, scale, before=None, after=None):
+    want, want_lse, p, absolute, size = oracle.attention(q, k, v, table, lens, starts, scale)
+    dt, dim = q.dtype, q.shape[-1]
+    n = table.shape[1] * k.shape[2]
+    # a score is a sum of dim products in fp32, scaled (two roundings more); its exponential is off by that and by two units
+    ds = (dim + 4) * F * size + 8 * F * (1 + size)
+    # out: each probability rounded to the element type, the sums in fp32, the result rounded; a half below 2^-14 is off by 2^-25
+    tol = _u(dt) * (absolute + want.abs()) + (2 * ds[:, None, :, None] + (64 + n / 16) * F) * absolute
+    if dt == HF:
+        tol = tol + 2.0 ** -25 * (n * 8 + 1)
+    assert bool(((out.cpu().double() - want).abs() <= tol).all()), float(((out.cpu().double() - want).abs() - tol).max())
+    finite = torch.isfinite(want_lse)
+    got = lse.cpu().double()
+    assert bool((got[~finite] == -math.inf).all())
+    assert bool(((got - want_lse).abs() <= ds + (64 + n / 16) * F + 4 * F * want_lse.abs())[finite].all())
+    if before is not None:
+        heads = k.shape[1]
+        w = p.view(p.shape[0], heads, -1, p.shape[-1])[..., :before.shape[-1]].sum(2)
+        rel = (2 * ds.view(ds.shape[0], heads, -1).max(-1).values + (64 + n / 16) * F)[..., None]
+        want_scores = before.double() + w
+        # (a weight is exp(s - lse) with s and the maximum up to `size` in size, and the sum of up to 16 of them and the score)
+        assert bool(((after.cpu().double() - want_scores).abs() <= rel * w + 18 * F * want_scores.abs()).all())
+        assert torch.equal(after.cpu()[w == 0], before[w == 0])
+
+
+CASES = [
+    # dt, B, heads, gs, dim, page, lens, starts
+    (BF, 1, 1, 1, 128, 16, [1], None),
+    (BF, 1, 2, 4, 128, 16, [17], None),
+    (HF, 3, 2, 7, 128, 16, [0, 1, 331], None),
+    (BF, 2, 1, 16, 128, 64, [640, 63], None),
+    (HF, 2, 3, 8, 64, 32, [100, 257], None),
+    (BF, 4, 2, 3, 64, 8, [9, 8, 7, 200], None),
+    (BF, 2, 2, 4, 128, 1, [5, 40], None),
+    (HF, 2, 1, 5, 128, 4, [50, 3], [13, 3]),
+    (BF, 4, 2, 4, 128, 16, [300, 300, 40, 16], [0, 290, 40, 15]),
+    (BF, 2, 1, 9, 64, 256, [1500, 700], [700, 0]),
+    (BF, 1, 2, 4, 128, 16, [5003], None),
+    (HF, 2, 1, 12, 128, 2, [1111, 0], [1, 0]),
+]
+
+
+@pytest.mark.parametrize("dt,B,heads,gs,dim,page,lens,starts", CASES)
+@pytest.mark.parametrize("scored", [False, True])
+def test_attention(dev, dt, B, heads, gs, dim, page, lens, starts, scored):
+    gen = torch.Generator().manual_seed(B * 1000 + dim + page + lens[0])
+    rows = max(lens) + 3
+    k, v, table = _pool(gen, dt, B, heads, dim, page, rows)
+    lens, starts = torch.tensor(lens, dtype=torch.int32), None if starts is None else torch.tensor(starts, dtype=torch.int32)
+    _spoil(k, v, table, lens, starts)
+    q = (2 * _randn(gen, B, 1, heads * gs, dim)).to(dt)
+    before = torch.rand(B, heads, table.shape[1] * page, generator=gen) if scored else None
+    on = lambda t: None if t is None else t.to(dev)  # noqa: E731
+    scores = on(before)
+    out, lse = kernels.paged_attention(on(q), on(k), on(v), on(table), on(lens), starts=on(starts), scores=scores,
+                                       return_softmax_lse=True)
+    _check_attention(q, k, v, table, lens, starts, out, lse, dim ** -0.5, before, scores)
+    again = kernels.paged_attention(on(q), on(k), on(v), on(table), on(lens), starts=on(starts))
+    assert torch.equal(again, out)   # no order of arrival in the result
+
+
+def test_attention_max_len_scale_and_strides(dev):
+    """Pages as [pages, rows, heads, dim], keys and values in one tensor, a table that is a part of a larger one, rows past max_len
+    and pages that are not there left out, a scale of its own."""
+    gen = torch.Generator().manual_seed(5)
+    B, heads, gs, dim, page, per = 3, 2, 6, 128, 16, 5
+    both = _randn(gen, B * per, 2, page, heads, dim).to(BF).to(dev)
+    k, v = both[:, 0].transpose(1, 2), both[:, 1].transpose(1, 2)
+    big = torch.randperm(B * per, generator=gen).view(B, per).to(torch.int32)
+    wide = torch.full((B, per + 3), -7, dtype=torch.int32)
+    wide[:, 1:per + 1] = big
+    wide[1, 2], wide[2, 1] = -1, B * per    # no such pages: rows 16 .. 31 of the second sequence, 0 .. 15 of the third
+    table = wide.to(dev)[:, 1:per + 1]
+    lens = torch.tensor([80, 33, 10], dtype=torch.int32)
+    q = _randn(gen, B, 1, heads * gs, dim).to(BF)
+    out, lse = kernels.paged_attention(q.to(dev), k, v, table, lens.to(dev), scale=0.2, max_len=77, return_softmax_lse=True)
+    _check_attention(q, k.cpu(), v.cpu(), table.cpu(), lens.clamp(max=77), None, out, lse, 0.2)
+    assert bool((out[2] == 0).all()) and bool((lse[2] == -math.inf).all())
+
+
+def test_attention_of_extreme_scores(dev):
+    """Scores far apart and all alike, keys with infinite elements, a sum that overflows without the running maximum."""
+    gen = torch.Generator().manual_seed(6)
+    k, v, table = _pool(gen, BF, 2, 1, 64, 16, 300, junk=False)
+    lens = torch.tensor([300, 290], dtype=torch.int32)
+    q = 60 * _randn(gen, 2, 1, 2, 64).to(BF)
+    out, lse = kernels.paged_attention(*(t.to(dev) for t in (q, k, v, table, lens)), return_softmax_lse=True)
+    _check_attention(q, k, v, table, lens, None, out, lse, 0.125)
+    same = kernels.paged_attention(*(t.to(dev) for t in (q * 0, k, v, table, lens)))
+    rows = oracle.rows_of(v, table[0], torch.arange(300))[0][0]
+    assert torch.allclose(same[0, 0, 0].cpu().double(), rows.mean(0), atol=2 * _u(BF) * float(rows.abs().mean(0).max()))
+    # a key of -inf where the query is positive: no weight
+    q = q.abs()
+    k[int(table[0, 2]), 0, 3] = -math.inf
+    out = kernels.paged_attention(*(t.to(dev) for t in (q, k, v, table, lens)))
+    assert bool(torch.isfinite(out).all())
+
+
+def test_attention_on_a_long_cache_past_32_bits(dev):
+    """Pages whose offsets pass 2^31 elements: only the last ones are looked at."""
+    heads, dim, page, pages = 2, 128, 256, 33000
+    k = torch.empty((pages, heads, page, dim), dtype=BF, device=dev)     # 4.3 GB, 2^31 elements and more
+    v = torch.empty_like(k)
+    gen = torch.Generator().manual_seed(7)
+    at = torch.tensor([[pages - 1, pages - 2, 32769]], dtype=torch.int32)
+    small_k, small_v = _randn(gen, 3, heads, page, dim).to(BF), _randn(gen, 3, heads, page, dim).to(BF)
+    k[at[0].long().to(dev)], v[at[0].long().to(dev)] = small_k.to(dev), small_v.to(dev)
+    q = _randn(gen, 1, 1, heads * 4, dim).to(BF)
+    lens = torch.tensor([700], dtype=torch.int32)
+    out, lse = kernels.paged_attention(q.to(dev), k, v, at.to(dev), lens.to(dev), return_softmax_lse=True)
+    _check_attention(q, small_k, small_v, torch.tensor([[0, 1, 2]]), lens, None, out, lse, dim ** -0.5)
+    key = _randn(gen, 1, 1, heads, dim).to(BF).to(dev)
+    kernels.paged_append(key, key, k, v, at.to(dev), lens.to(dev))
+    assert torch.equal(k[32769, :, 700 - 512], key[0, 0])
+
+
+# ------------------------------------------------------------------------------------------------ append
+def _append_state(gen, dt, B, heads, dim, page, budget, lens, seen, sinks, recent, ties):
+    k, v, table = _pool(gen, dt, B, heads, dim, page, budget, junk=False)
+    scores = torch.rand(B, heads, budget, generator=gen)
+    if ties:
+        scores = (scores * 4).floor() - 1      # -1, 0, 1, 2: rows share their score
+        scores[scores == 0] = -0.0
+    positions = torch.stack([torch.randperm(max(seen), generator=gen)[:budget].sort().values[torch.randperm(budget, generator=gen)]
+                             for _ in range(B * heads)]).view(B, heads, budget).to(torch.int32)
+    return k, v, table, scores, positions, torch.tensor(lens, dtype=torch.int32), torch.tensor(seen, dtype=torch.int32)
+
+
+@pytest.mark.parametrize("dt,B,heads,dim,page,budget,lens,seen,sinks,recent,ties", [
+    (BF, 1, 1, 128, 16, 1, [0], [0], 0, 0, False),
+    (BF, 1, 1, 128, 16, 1, [1], [9], 0, 0, False),
+    (HF, 3, 2, 64, 8, 37, [37, 36, 0], [90, 40, 0], 4, 5, False),
+    (BF, 2, 3, 128, 32, 700, [700, 700], [3000 - 100, 800], 4, 64, True),
+    (BF, 2, 2, 128, 64, 4111, [4111, 5000], [9000, 7000], 0, 0, True),
+    (HF, 1, 8, 64, 1, 64, [64], [64], 20, 43, False),
+    (BF, 1, 2, 64, 256, 20000, [20000], [30000], 4, 512, False),
+])
+def test_append(dev, dt, B, heads, dim, page, budget, lens, seen, sinks, recent, ties):
+    gen = torch.Generator().manual_seed(budget + page)
+    k, v, table, scores, positions, lens, seen = _append_state(gen, dt, B, heads, dim, page, budget, lens,
+                                                               [max(x, budget) for x in seen], sinks, recent, ties)
+    key = _randn(gen, B, 1, heads, dim + 8).to(dt)[..., :dim]    # strided rows
+    value = _randn(gen, B, heads, 1, dim).to(dt).transpose(1, 2)
+    d = [t.to(dev) for t in (k, v, table, lens, scores, positions, seen)]
+    held = torch.full((B,), -5, dtype=torch.int32, device=dev)
+    wide = torch.empty(B, 1, heads, dim + 8, dtype=dt, device=dev)[..., :dim].copy_(key)
+    kernels.paged_append(wide, value.to(dev), d[0], d[1], d[2], d[3], held, scores=d[4], positions=d[5], token_positions=d[6],
+                         budget=budget, sinks=sinks, recent=recent)
+    for b in range(B):
+        n = min(int(lens[b]), budget)
+        for h in range(heads):
+            r = n if n < budget else oracle.victim(scores[b, h], positions[b, h], n, int(seen[b]), sinks, recent)
+            p = int(table[b, r // page])
+            k[p, h, r % page], v[p, h, r % page] = key[b, 0, h], value[b, 0, h]
+            scores[b, h, r], positions[b, h, r] = 0.0, seen[b]
+        assert int(held[b]) == min(n + 1, budget)
+    for got, want in zip((d[0], d[1], d[4], d[5]), (k, v, scores, positions)):
+        assert torch.equal(got.cpu(), want)
+
+
+def test_append_without_scores_and_with_odd_ones(dev):
+    """Plain appends leave a full sequence as it is; NaN counts as the highest score, -inf as the lowest; where every row stays, the
+    first one goes; a page that is not there takes nothing."""
+    gen = torch.Generator().manual_seed(8)
+    k, v, table, scores, positions, lens, seen = _append_state(gen, BF, 4, 1, 64, 16, 32, [31, 32, 7, 16], [40, 40, 40, 40], 0, 0, False)
+    table[3, 1] = -1
+    key = _randn(gen, 4, 1, 1, 64).to(BF)
+    d = [t.to(dev) for t in (key, key, k, v, table, lens)]
+    held = torch.zeros(4, dtype=torch.int32, device=dev)
+    kernels.paged_append(*d, held)
+    for b, r in ((0, 31), (2, 7)):
+        k[int(table[b, r // 16]), :, r % 16] = key[b, 0]
+    assert torch.equal(d[2].cpu(), k) and held.tolist() == [32, 32, 8, 17]
+    lens = torch.full((4,), 32, dtype=torch.int32)
+    scores[0, 0, :] = math.nan
+    scores[0, 0, 9] = math.inf
+    scores[1, 0, 21] = -math.inf
+    positions[2] = 1
+    full = [t.to(dev) for t in (key, key, k, v, table, lens)]
+    s, p = scores.to(dev), positions.to(dev)
+    kernels.paged_append(*full, scores=s, positions=p, token_positions=seen.to(dev), sinks=2, recent=3, budget=32)
+    for b in range(3):
+        r = oracle.victim(scores[b, 0], positions[b, 0], 32, 40, 2, 3)
+        assert int(p[b, 0, r]) == 40 and float(s[b, 0, r]) == 0.0 and int((p[b, 0].cpu() != positions[b, 0]).sum()) <= 1
+    assert oracle.victim(scores[2, 0], positions[2, 0], 32, 40, 2, 3) == 0
+
+
+# ------------------------------------------------------------------------------------------------ fill
+@pytest.mark.parametrize("dt,B,T,heads,dim,page,budget,lens,sinks,recent,weights", [
+    (BF, 1, 1, 1, 128, 16, None, None, 0, 0, None),
+    (HF, 2, 37, 3, 64, 8, None, [37, 0], 0, 0, None),
+    (BF, 3, 300, 2, 128, 16, 64, [300, 64, 65], 4, 16, "any"),
+    (BF, 2, 2500, 2, 64, 32, 1000, None, 0, 0, "few"),
+    (HF, 1, 5000, 1, 128, 64, 4999, None, 4, 4000, "few"),
+    (BF, 1, 1100, 2, 128, 4, 16, [1100], 8, 8, "any"),
+    (BF, 2, 1030, 1, 128, 16, 100, [1030, 99], 1, 0, "zero"),
+    (BF, 1, 4097, 2, 64, 256, 1, None, 0, 0, "odd"),
+    (BF, 1, 70000, 2, 64, 256, 9000, None, 4, 64, "any"),
+])
+def test_fill(dev, dt, B, T, heads, dim, page, budget, lens, sinks, recent, weights):
+    gen = torch.Generator().manual_seed(T + page)
+    room = budget or T
+    k, v, table = _pool(gen, dt, B, heads, dim, page, room, junk=False)
+    key, value = _randn(gen, B, T, heads, dim).to(dt), _randn(gen, B, T, heads, 2, dim).to(dt)[:, :, :, 1]
+    lens_t = None if lens is None else torch.tensor(lens, dtype=torch.int32)
+    w = None
+    if weights:
+        w = torch.exp(4 * _randn(gen, B, heads, T)) if weights in ("any", "odd") else torch.zeros(B, heads, T)
+        if weights == "few":
+            w = (torch.rand(B, heads, T, generator=gen) * 5).floor()
+        if weights == "odd":
+            w[..., ::7], w[..., 5], w[..., 4000] = -1.0, math.inf, math.nan
+    scores = torch.full((B, heads, room), 3.0) if w is not None else None
+    positions = torch.full((B, heads, room), -9, dtype=torch.int32)
+    on = lambda t: None if t is None else t.to(dev)  # noqa: E731
+    d = [on(t) for t in (k, v, table, scores, positions)]
+    held = torch.full((B,), -5, dtype=torch.int32, device=dev)
+    wide = torch.empty(B, T, heads, 2, dim, dtype=dt, device=dev)
+    wide[:, :, :, 1] = value.to(dev)
+    kernels.paged_fill(key.to(dev), wide[:, :, :, 1], d[0], d[1], d[2], held, seqlens=on(lens_t), weights=on(w), scores=d[3],
+                       positions=d[4], budget=budget, sinks=sinks, recent=recent)
+    for b in range(B):
+        n = T if lens is None else lens[b]
+        for h in range(heads):
+            rows = torch.tensor(oracle.kept(None if w is None else w[b, h].tolist(), n, room, sinks, recent), dtype=torch.long)
+            r = torch.arange(rows.numel())
+            at = table[b].long()[r // page]
+            k[at, h, r % page], v[at, h, r % page] = key[b, rows, h], value[b, rows, h]
+            positions[b, h, r] = rows.to(torch.int32)
+            if scores is not None:
+                scores[b, h, r] = w[b, h, rows]
+        assert int(held[b]) == min(n, room)
+    for got, want in zip((d[0], d[1], d[4]), (k, v, positions)):
+        assert torch.equal(got.cpu(), want)
+    if scores is not None:
+        assert torch.equal(d[3].cpu().nan_to_num(-77), scores.nan_to_num(-77))
+
+
+# ------------------------------------------------------------------------------------------------ weights of a prompt
+@pytest.mark.parametrize("dt,B,T,W,heads,gs,dim,lens", [
+    (BF, 1, 1, 1, 1, 1, 128, None),
+    (HF, 2, 33, 33, 1, 3, 64, None),
+    (BF, 3, 70, 9, 2, 4, 128, [70, 5, 0]),
+    (BF, 1, 260, 40, 1, 7, 128, None),
+    (HF, 2, 515, 16, 2, 16, 64, [515, 129]),
+    (BF, 1, 130, 130, 2, 2, 128, [129]),
+    (BF, 1, 3300, 3, 1, 5, 64, None),
+])
+def test_prompt_weights(dev, dt, B, T, W, heads, gs, dim, lens):
+    gen = torch.Generator().manual_seed(T + W)
+    q, key = (2 * _randn(gen, B, W, heads * gs, dim)).to(dt), _randn(gen, B, T, heads, dim).to(dt)
+    lens_t = None if lens is None else torch.tensor(lens, dtype=torch.int32)
+    want, size = oracle.weigh(q, key, lens_t, dim ** -0.5)
+    if lens is not None:   # what lies behind a prompt's end has no say
+        for b, n in enumerate(lens):
+            key[b, n:] = math.nan
+            q[b, :max(0, W - n)] = math.inf
+    # heads first, as a transposed view, and a part of a wider tensor
+    kd = key.transpose(1, 2).contiguous().to(dev).transpose(1, 2)
+    qd = torch.empty(B, W, heads * gs, dim + 8, dtype=dt, device=dev)[..., :dim].copy_(q)
+    got = kernels.attention_weights(qd, kd, seqlens=None if lens is None else lens_t.to(dev))
+    # relative errors: of the exponentials (their arguments are sums of dim products in fp32, up to `size`, less a log-sum-exp of
+    # that order), of the sum of T terms in the lse and of W * gs terms here, all in fp32
+    rel = 4 * (dim + 12) * F * (1 + size) + (64 + T / 32 + W * gs / 32) * F
+    assert bool(((got.cpu().double() - want).abs() <= rel * want + 1e-30).all()), \
+        float(((got.cpu().double() - want).abs() / want.clamp(min=1e-30)).max())
+    again = kernels.attention_weights(q.to(dev), key.to(dev), seqlens=None if lens is None else lens_t.to(dev))
+    assert torch.equal(again, got)

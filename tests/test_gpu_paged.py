@@ -292,6 +292,9 @@ def test_fill(dev, dt, B, T, heads, dim, page, budget, lens, sinks, recent, weig
     (HF, 2, 515, 16, 2, 16, 64, [515, 129]),
     (BF, 1, 130, 130, 2, 2, 128, [129]),
     (BF, 1, 3300, 3, 1, 5, 64, None),
+    (BF, 1, 700, 700, 1, 4, 128, None),
+    (HF, 2, 600, 300, 1, 3, 64, [600, 299]),
+    (BF, 1, 1600, 40, 2, 16, 128, [1599]),
 ])
 def test_prompt_weights(dev, dt, B, T, W, heads, gs, dim, lens):
     gen = torch.Generator().manual_seed(T + W)
@@ -313,3 +316,32 @@ def test_prompt_weights(dev, dt, B, T, W, heads, gs, dim, lens):
         float(((got.cpu().double() - want).abs() / want.clamp(min=1e-30)).max())
     again = kernels.attention_weights(q.to(dev), key.to(dev), seqlens=None if lens is None else lens_t.to(dev))
     assert torch.equal(again, got)
+
+
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 3.0])
+def test_prompt_weights_scales(dev, scale):
+    gen = torch.Generator().manual_seed(9)
+    q, key = _randn(gen, 1, 50, 3, 64).to(BF), _randn(gen, 1, 300, 1, 64).to(BF)
+    want, size = oracle.weigh(q, key, None, scale)
+    got = kernels.attention_weights(q.to(dev), key.to(dev), scale=scale)
+    rel = 4 * (64 + 12) * F * (1 + size.abs()) + (64 + 300 / 32 + 150 / 32) * F
+    assert bool(((got.cpu().double() - want).abs() <= rel * want + 1e-30).all())
+
+
+def test_prompt_weights_far_apart(dev):
+    """Scores that rise along the prompt by more than an exponential of fp32 can tell, and fall."""
+    gen = torch.Generator().manual_seed(10)
+    T = 900
+    key = torch.zeros(1, T, 2, 64)
+    key[0, :, 0, 0] = torch.arange(T) / 4       # 0 .. 225, exact in bfloat16
+    key[0, :, 0, 0] = key[0, :, 0, 0].floor()
+    key[0, :, 1, 0] = -key[0, :, 0, 0]
+    key[..., 1] = _randn(gen, 1, T, 2)
+    key = key.to(BF)
+    q = torch.zeros(1, 7, 2, 64)
+    q[..., 0], q[..., 1] = 16.0, 1.0
+    want, size = oracle.weigh(q.to(BF), key, None, 1.0)
+    got = kernels.attention_weights(q.to(BF).to(dev), key.to(dev), scale=1.0).cpu().double()
+    # (each score is exact up to a rounding of its sum and one of its product with 1 / ln 2: 3 roundings of 3600 / ln 2 here)
+    rel = 8 * F * (1 + size) * 1.5 + 64 * F
+    assert bool(((got - want).abs() <= rel * want + 1e-30).all())

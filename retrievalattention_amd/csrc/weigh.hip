@@ -7,19 +7,19 @@
 // l holds one column of the product, l % 32, and of its rows 8 (i / 4) + 4 (l / 32) + i % 4 as accumulator i: with the columns as
 // columns the sums over keys stay in the lane until all tiles are done, with the keys as columns those over columns do.
 //
-// A wave keeps 64 columns in registers, and a workgroup of four streams the keys through LDS, 64 at a time straight from memory,
-// three tiles ahead.  The matrix cores (32 cycles to an instruction) and the exponentials (8, and 4 each for the product with
-// its offset and the addition) take the same time, 256 cycles for a tile of 128 dims, so one tile's products are issued between
-// the exponentials of the tile before.
+// A wave keeps 32 columns in registers, and a workgroup of eight streams the keys through LDS, 64 at a time straight from memory,
+// two tiles ahead.  One tile's products are issued between the exponentials of the tile before: matrix instructions, exponentials
+// and their products and sums in such turns take 400 cycles a tile of 128 dims (registers alone, two waves and more to a SIMD;
+// one wave 570; the matrix instructions alone 300, the rest 275).
 #include <math.h>
 
 #include "ri_common.h"
 
-#define WG_WAVES 4
-#define WG_BLOCK (64 * WG_WAVES)   // columns of a workgroup
+#define WG_COLS 256                // columns of a workgroup of the first pass, to a multiple of which they are padded
+#define WG_SUM_COLS 128            // and of the second
 #define WG_TILE 64                 // rows of a streamed tile
 #define WG_BUFFERS 3
-#define WG_ROWS 1024               // keys of a split at most
+#define WG_ROWS 4096               // keys of a split at most
 #define WG_LOG2E 1.4426950408889634f
 
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
@@ -82,219 +82,238 @@ __device__ __forceinline__ void weigh_wait() { asm volatile("s_waitcnt vmcnt(%0)
 __device__ __forceinline__ void weigh_barrier() { asm volatile("s_barrier" ::: "memory"); }
 
 // A streamed tile in LDS: row r's piece p (16 bytes) lies at place p ^ (r % pieces) of the row, so that neither the 32 rows that
-// a wave reads a piece of nor the loads, a row by a row's lanes, meet in a bank.  offset(r): byte offset of row r's start in
-// memory from `base`; a wave loads a quarter of the rows, WG_LOADS<D> instructions.
-template <int D>
-constexpr int WG_LOADS = WG_TILE * D * 2 / (1024 * WG_WAVES);
-template <int D, typename Offset>
-__device__ __forceinline__ void weigh_stage(const void* base, uint16_t* tile, int wave, Offset&& offset) {
-  constexpr int PP = D / 8, RW = 64 / PP;
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int i = 0; i < WG_LOADS<D>; ++i) {
-    const int r0 = (wave * WG_LOADS<D> + i) * RW, r = r0 + lane / PP;
-    weigh_dma16(base, offset(r) + (((lane % PP) ^ (r % PP)) << 4), __builtin_amdgcn_readfirstlane(weigh_lds(tile + r0 * D)));
-  }
+// a wave reads a piece of nor the loads, a row by a row's lanes, meet in a bank.  Load i of a wave: this lane's row
+// of the tile and the byte offset of its piece in the row.
+template <int D, int WAVES>
+__device__ __forceinline__ int weigh_row(int wave, int i) {
+  return (wave + i * WAVES) * (512 / D) + ((threadIdx.x & 63) / (D / 8));
 }
-// lane's operand kk of the 32 rows from `sub` on: row sub + lane % 32, dims 16 kk + 8 (lane / 32) ..
-template <int D>
-__device__ __forceinline__ uint4 weigh_operand(const uint16_t* tile, int sub, int kk) {
-  constexpr int PP = D / 8;
-  const int lane = threadIdx.x & 63, r = lane & 31;
-  return *reinterpret_cast<const uint4*>(tile + (sub + r) * D + (((2 * kk + (lane >> 5)) ^ (r % PP)) << 3));
+template <int D, int WAVES>
+__device__ __forceinline__ uint32_t weigh_piece(int wave, int i) {
+  return (((threadIdx.x & 63) % (D / 8)) ^ (weigh_row<D, WAVES>(wave, i) % (D / 8))) << 4;
 }
 
-// Waits for a wave's own operand, so that no wait for it stands between the counted ones for the tiles.
-template <int KK>
-__device__ __forceinline__ void weigh_arrived(uint4 (&x)[2][KK]) {
-#pragma unroll
-  for (int t = 0; t < 2; ++t)
-#pragma unroll
-    for (int kk = 0; kk < KK; ++kk) asm volatile("" : "+v"(x[t][kk].x), "+v"(x[t][kk].y), "+v"(x[t][kk].z), "+v"(x[t][kk].w));
-  weigh_wait<0>();
+// The last key that the columns of part `super` of the second pass see.
+__device__ __forceinline__ int weigh_last_key(const WeighParams& P, int n, int super, int block) {
+  return n - P.W + min((super + 1) * P.per * block - 1, P.cols - 1) / P.gs;
 }
 
-// The product of one tile beside the exponentials of the one before: eight (D = 64: four) matrix instructions, each followed by
-// a share of the sixteen exponentials and their additions.
-template <int KK>
-__device__ __forceinline__ void weigh_interleave() {
-#pragma unroll
-  for (int kk = 0; kk < KK; ++kk) {
-    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);             // matrix product
-    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);             // LDS read
-    __builtin_amdgcn_sched_group_barrier(0x400, 16 / KK, 0);       // exponentials
-    __builtin_amdgcn_sched_group_barrier(0x002, 2 * 16 / KK, 0);   // their products and sums
-  }
-}
-
-// One pass over the keys [j0, j1) of split blockIdx.z of group blockIdx.x.
-// SUM false: the lse.  Columns of block gridDim.y - 1 - blockIdx.y (those that see most keys first), as columns of the product;
+// One pass over the keys [j0, j1) of split blockIdx.z of group blockIdx.x, of which the columns [32 wave, 32 wave + 32) of
+// a block of 32 WAVES see some.
+// SUM false: the lse, of a block's columns as columns of the product;
 // m and l of a lane: its reference and the sum of exponentials relative to it, over its own keys.  The reference is the maximum of
 // the first tile that the column sees, and moves only where a tile's sum passes 2^100: until then neither the sums nor their
 // precision suffer, and a score costs a product with its offset, an exponential and an addition.
-// SUM true: the sums over the columns of `per` blocks from blockIdx.y * per on, as rows of the product, so that the columns add
-// up in the lane; a wave keeps its sums of the split's keys in LDS.
-template <int D, bool HALF, bool SUM>
-__global__ __launch_bounds__(64 * WG_WAVES, 2) void weigh_kernel(WeighParams P) {
-  constexpr int KK = D / 16, L = WG_LOADS<D>;
+// SUM true: the sums over the columns of `per` blocks, as rows of the product, so that the columns add
+// up in the lane; the waves leave theirs in LDS, where one of them adds up a tile's behind the barrier that follows.
+template <int D, bool HALF, bool SUM, int WAVES, int OCC>
+__global__ __launch_bounds__(64 * WAVES, OCC) void weigh_kernel(WeighParams P) {
+  constexpr int BLOCK = 32 * WAVES, LOADS = WG_TILE * D * 2 / (1024 * WAVES), KK = D / 16, EX = 16 / KK, RING = 4;   // EX: exponentials to a product; RING: operands read ahead
   __shared__ __attribute__((aligned(16))) uint16_t sh[WG_BUFFERS][WG_TILE * D];
-  __shared__ __attribute__((aligned(16))) float sh_lse[SUM ? WG_BLOCK : 4];
-  extern __shared__ float sh_sum[];   // [WG_WAVES][rows]
+  __shared__ __attribute__((aligned(16))) float sh_lse[SUM ? BLOCK : 4];
+  __shared__ float sh_part[SUM ? WG_BUFFERS : 1][SUM ? WAVES : 1][WG_TILE];
+  extern __shared__ float sh_sum[];   // [rows], with several blocks
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = blockIdx.x, b = g / P.heads, head = g - b * P.heads;
   const int n = weigh_len(P, b), first = n - P.W;                   // first: the first query's token
-  const int blocks = P.cols_pad / WG_BLOCK;
-  const int block0 = SUM ? blockIdx.y * P.per : gridDim.y - 1 - blockIdx.y, block1 = SUM ? min(block0 + P.per, blocks) : block0 + 1;
+  const int blocks = (P.cols + BLOCK - 1) / BLOCK;
+  const int super = gridDim.y - 1 - blockIdx.y;                     // (the columns that see most keys first)
+  const int block0 = SUM ? super * P.per : super, block1 = SUM ? min(block0 + P.per, blocks) : block0 + 1;
   const int j0 = blockIdx.z * P.rows, jn = min(j0 + P.rows, n);
   const uint16_t* const keys = P.key + b * P.kb + head * P.kh;
-  const uint32_t stride = (uint32_t)P.kt * 2;
+  uint32_t at[LOADS];   // of this lane's piece of a tile's rows
+#pragma unroll
+  for (int i = 0; i < LOADS; ++i) at[i] = weigh_row<D, WAVES>(wave, i) * ((uint32_t)P.kt * 2) + weigh_piece<D, WAVES>(wave, i);
   const auto stage = [&](int t) {
     const int j = j0 + t * WG_TILE;
-    weigh_stage<D>(keys + j * P.kt, sh[t % WG_BUFFERS], wave, [&](int r) { return (uint32_t)min(r, n - 1 - j) * stride; });
+    const uint16_t* const from = keys + j * P.kt;
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {   // (past the last key: that one)
+      const uint32_t o = j + WG_TILE <= n ? at[i]
+                                          : (uint32_t)min(weigh_row<D, WAVES>(wave, i), n - 1 - j) * ((uint32_t)P.kt * 2) + weigh_piece<D, WAVES>(wave, i);
+      weigh_dma16(from, o, __builtin_amdgcn_readfirstlane(weigh_lds(sh[t % WG_BUFFERS]) + (wave + i * WAVES) * 1024));
+    }
   };
-  float* const mine_sum = sh_sum + wave * P.rows;
-  if (SUM)
-    for (int i = lane; i < P.rows; i += 64) mine_sum[i] = 0.f;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  const uint16_t* operand_at[KK];   // operand kk of a tile's first 32 rows: row lane % 32, dims 16 kk + 8 (lane / 32) ..
+#pragma unroll
+  for (int kk = 0; kk < KK; ++kk)
+    operand_at[kk] = &sh[0][(lane & 31) * D + (((2 * kk + (lane >> 5)) ^ (lane % (D / 8))) << 3)];
+  float* const to = !SUM ? nullptr : P.supers > 1 ? P.part + ((size_t)g * P.supers + super) * P.T : P.out + (size_t)g * P.T;
+  if (SUM && P.per > 1)
+    for (int i = threadIdx.x; i < P.rows; i += 64 * WAVES) sh_sum[i] = 0.f;
+  float m = -INFINITY, l = 0.f;
 
   for (int block = block0; block < block1; ++block) {
-    const int colw = block * WG_BLOCK + wave * 64;
-    const int j1 = min(jn, first + min(block * WG_BLOCK + WG_BLOCK - 1, P.cols - 1) / P.gs + 1);   // (the last key of the block)
+    const int colw = block * BLOCK + wave * 32;
+    const int j1 = min(jn, first + min(block * BLOCK + BLOCK - 1, P.cols - 1) / P.gs + 1);   // (the last key of the block)
     if (j0 >= j1) continue;
     const int tiles = (j1 - j0 + WG_TILE - 1) / WG_TILE, subs = (j1 - j0 + 31) / 32;
     if (SUM) {   // the block's lse, joined from its splits where nobody has done so before
-      __syncthreads();
-      const int col = block * WG_BLOCK + threadIdx.x;
-      sh_lse[threadIdx.x] = P.joined ? P.lse[(size_t)g * P.cols_pad + col] : weigh_join(P, g, col, 0, 1);
+      if ((int)threadIdx.x < BLOCK) {
+        const int col = block * BLOCK + threadIdx.x;
+        sh_lse[SUM ? threadIdx.x : 0] = P.joined ? P.lse[(size_t)g * P.cols_pad + col] : weigh_join(P, g, col, 0, 1);
+      }
       __syncthreads();
     }
-    uint4 q[2][KK];
-    int low[2];                 // last key of each tile's first column
-    f32x16_t off[2];            // SUM: minus the lse of the rows
-    int mine[2];                // else: last key of the lane's column
+    uint4 q[KK];
+    f32x16_t off;               // SUM: minus the lse of the rows
+    const int col = min(colw + (lane & 31), P.cols - 1), qi = col / P.gs;
+    const int low = first + min(colw, P.cols - 1) / P.gs, mine = first + qi;   // last keys of the tile's first and the lane's column
+    {
+      const uint16_t* from = P.q + b * P.qb + qi * P.qt + (head * P.gs + col - qi * P.gs) * P.qh + 8 * (lane >> 5);
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int c = colw + 32 * t, col = min(c + (lane & 31), P.cols - 1), i = col / P.gs;
-      mine[t] = first + i;
-      low[t] = first + min(c, P.cols - 1) / P.gs;
-      const uint16_t* at = P.q + b * P.qb + i * P.qt + (head * P.gs + col - i * P.gs) * P.qh + 8 * (lane >> 5);
-#pragma unroll
-      for (int kk = 0; kk < KK; ++kk) q[t][kk] = ri_ld16(at + 16 * kk);
+      for (int kk = 0; kk < KK; ++kk) q[kk] = ri_ld16(from + 16 * kk);
       if (SUM) {
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          const float4 o = *reinterpret_cast<const float4*>(&sh_lse[wave * 64 + 32 * t + 8 * x + 4 * (lane >> 5)]);
-          off[t][4 * x] = -o.x; off[t][4 * x + 1] = -o.y; off[t][4 * x + 2] = -o.z; off[t][4 * x + 3] = -o.w;
+          const float4 o = *reinterpret_cast<const float4*>(&sh_lse[wave * 32 + 8 * x + 4 * (lane >> 5)]);
+          off[4 * x] = -o.x; off[4 * x + 1] = -o.y; off[4 * x + 2] = -o.z; off[4 * x + 3] = -o.w;
         }
       }
+      // waited for here, so that no wait for them stands between those for the tiles
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) asm volatile("" : "+v"(q[kk].x), "+v"(q[kk].y), "+v"(q[kk].z), "+v"(q[kk].w));
     }
-    weigh_arrived(q);
+    weigh_wait<0>();
     stage(0);
-    if (tiles > 1) stage(1);
-    if (tiles > 2) stage(2);
-    if (tiles > 2) weigh_wait<2 * L>();
-    else if (tiles > 1) weigh_wait<L>();
-    else weigh_wait<0>();
+    if (tiles > 1) {
+      stage(1);
+      weigh_wait<LOADS>();
+    } else {
+      weigh_wait<0>();
+    }
     weigh_barrier();
-    uint4 a[KK];
-#pragma unroll
-    for (int kk = 0; kk < KK; ++kk) a[kk] = weigh_operand<D>(sh[0], 0, kk);
-    const auto product = [&](int t, int kk, f32x16_t c) {
-      return SUM ? weigh_mfma<HALF>(q[t][kk], a[kk], c) : weigh_mfma<HALF>(a[kk], q[t][kk], c);
+    uint4 a[RING];
+    const auto operand = [&](int buf, int sub, int kk) {
+      return *reinterpret_cast<const uint4*>(operand_at[kk] + (buf * WG_TILE + sub * 32) * D);
     };
+#pragma unroll
+    for (int kk = 0; kk < RING; ++kk) a[kk] = operand(0, 0, kk);
     const f32x16_t zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    f32x16_t s[2];
-    s[0] = zero;
+    f32x16_t s;                 // the scores of the sub-tile before
 #pragma unroll
-    for (int kk = 0; kk < KK; ++kk) s[0] = product(0, kk, s[0]);
-    for (int u = 0; u < subs; ++u) {
-      const int j = j0 + 32 * u;
-      if ((u & 1) && u + 1 < subs) {   // the next sub-tile is the next tile's first; nobody reads this tile any more
-        const int t = u >> 1;
-        if (t + 2 < tiles) weigh_wait<L>();
-        else weigh_wait<0>();
-        weigh_barrier();
-        if (t + 3 < tiles) stage(t + 3);
-      }
-      const int next = min(u + 1, subs - 1);
-      const uint16_t* const tile = sh[(next >> 1) % WG_BUFFERS];
-      float both = 0.f;
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        float scale2 = P.scale2;
-        if (j + 31 > low[t]) {   // some column does not see every key
-          if (SUM) {
-            const int key = j + (lane & 31), c = colw + 32 * t, i0 = c / P.gs, at = c - i0 * P.gs + 4 * (lane >> 5);
-            const uint32_t inv = 65536 / P.gs + 1;   // (exact for what is divided here: less than 48 by up to 16)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const int last = first + i0 + (int)(((uint32_t)(at + 8 * (i >> 2) + (i & 3)) * inv) >> 16);
-              s[t][i] = key > last ? -INFINITY : s[t][i] * scale2;
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) s[t][i] = j + weigh_key_of(i, lane) > mine[t] ? -INFINITY : s[t][i] * scale2;
-          }
-          scale2 = 1.f;
-        }
-        // tile t's exponentials beside the product of the other tile (of the next sub-tile behind t = 1)
-        f32x16_t p = zero;
-        float sum = 0.f, x = 0.f;
-#pragma unroll
-        for (int kk = 0; kk < KK; ++kk) {
-          p = product(1 - t, kk, p);
-          if (t == 0) a[kk] = weigh_operand<D>(tile, (next & 1) * 32, kk);
-        }
-#pragma unroll
-        for (int i = 0; i < 16; i += 2) {   // (two sums, so that an addition does not wait for the one before)
-          sum += __builtin_amdgcn_exp2f(fmaf(s[t][i], scale2, SUM ? off[t][i] : -m[t]));
-          x += __builtin_amdgcn_exp2f(fmaf(s[t][i + 1], scale2, SUM ? off[t][i + 1] : -m[t]));
-        }
-        sum += x;
-        weigh_interleave<KK>();
-        if (SUM) {
-          both += sum;
-        } else {
-          if (__builtin_amdgcn_ballot_w64(!(sum < 0x1p100f))) {
-            float most = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) most = fmaxf(most, s[t][i] * scale2);
-            const float mn = fmaxf(m[t], most), ref = mn == -INFINITY ? 0.f : mn;
-            l[t] *= __builtin_amdgcn_exp2f(m[t] - ref);
-            m[t] = mn;
-            sum = 0.f;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) sum += __builtin_amdgcn_exp2f(fmaf(s[t][i], scale2, -ref));
-          }
-          l[t] += sum;
-        }
-        s[1 - t] = p;
-      }
+    for (int i = 0; i < 16; ++i) s[i] = -INFINITY;
+
+    // keys from j on that a column does not see weigh nothing; the factor that the scores still want
+    const auto mask = [&](int j) {
+      if (j + 31 <= low) return P.scale2;
+      int here = lane;
+      asm volatile("" : "+v"(here));   // (what follows is rare: nothing of it is to be kept in registers for it)
       if (SUM) {
-        both = ri_xor_sum<32>(both);
-        if (lane < 32) mine_sum[32 * u + lane] += both;
+        const int key = j + (here & 31), i0 = colw / P.gs, o = colw - i0 * P.gs + 4 * (here >> 5);
+        const uint32_t inv = 65536 / P.gs + 1;   // (exact for what is divided here: less than 48 by up to 16)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int last = first + i0 + (int)(((uint32_t)(o + 8 * (i >> 2) + (i & 3)) * inv) >> 16);
+          s[i] = key > last ? -INFINITY : s[i] * P.scale2;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = j + weigh_key_of(i, here) > mine ? -INFINITY : s[i] * P.scale2;
+      }
+      return 1.f;
+    };
+    // the sum of a sub-tile's exponentials, to where it belongs
+    const auto finish = [&](float sum, float scale2, int slot, int sub) {
+      if (SUM) {
+        sh_part[SUM ? slot : 0][SUM ? wave : 0][sub * 32 + (lane & 31)] = ri_xor_sum<32>(sum);
+        return;
+      }
+      if (__builtin_amdgcn_ballot_w64(!(sum < 0x1p100f))) {
+        float most = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) most = fmaxf(most, s[i] * scale2);
+        const float mn = fmaxf(m, most), ref = mn == -INFINITY ? 0.f : mn;
+        l *= __builtin_amdgcn_exp2f(m - ref);
+        m = mn;
+        sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sum += __builtin_amdgcn_exp2f(fmaf(s[i], scale2, -ref));
+      }
+      l += sum;
+    };
+    const auto add_tile = [&](int t) {   // (a tile is the same wave's in every block)
+      if (wave == t % WAVES && t * WG_TILE + lane < subs * 32) {
+        float x = 0.f;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) x += sh_part[SUM ? t % WG_BUFFERS : 0][SUM ? w : 0][lane];
+        if (P.per > 1) sh_sum[t * WG_TILE + lane] += x;
+        else if (j0 + t * WG_TILE + lane < jn) to[j0 + t * WG_TILE + lane] = x;
+      }
+    };
+
+    for (int t0 = 0; t0 < tiles; t0 += WG_BUFFERS) {
+#pragma unroll
+      for (int buf = 0; buf < WG_BUFFERS; ++buf) {   // (unrolled: the buffer is in the offset of every LDS access)
+        const int t = t0 + buf;
+        if (t >= tiles) break;
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub) {
+          const int u = 2 * t + sub;
+          if (u >= subs) break;
+          if (sub && t + 1 < tiles) {   // the operands read ahead are the next tile's; nobody reads the one before this any more
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            if (t + 2 < tiles) stage(t + 2);
+            if (SUM && t) add_tile(t - 1);
+          }
+          // this sub-tile's product beside the exponentials of the one before
+          const float scale2 = u ? mask(j0 + 32 * u - 32) : 1.f;
+          f32x16_t p = zero;
+          float sum = 0.f, x = 0.f, e[EX];
+          const auto add = [&]() {   // (two sums, so that an addition does not wait for the one before)
+#pragma unroll
+            for (int i = 0; i < EX; i += 2) { sum += e[i]; x += e[i + 1]; }
+          };
+#pragma unroll
+          for (int kk = 0; kk < KK; ++kk) {
+            uint4& from = a[kk % RING];
+            p = SUM ? weigh_mfma<HALF>(q[kk], from, p) : weigh_mfma<HALF>(from, q[kk], p);
+            from = kk + RING < KK ? operand(buf, sub, kk + RING)
+                                  : sub ? operand((buf + 1) % WG_BUFFERS, 0, kk + RING - KK) : operand(buf, 1, kk + RING - KK);
+            if (kk) add();
+#pragma unroll
+            for (int i = 0; i < EX; ++i)
+              e[i] = __builtin_amdgcn_exp2f(fmaf(s[EX * kk + i], scale2, SUM ? off[EX * kk + i] : -m));
+            // (the next product cannot move in front of these exponentials, nor they behind it)
+#pragma unroll
+            for (int i = 0; i < EX; i += 2) asm volatile("" : "+v"(e[i]), "+v"(e[i + 1]), "+v"(q[(kk + 1) % KK].x));
+            __builtin_amdgcn_sched_barrier(0);
+          }
+          add();
+          if (u) finish(sum + x, scale2, sub ? buf : (buf + WG_BUFFERS - 1) % WG_BUFFERS, sub ^ 1);
+          s = p;
+        }
       }
     }
-    if (SUM) weigh_barrier();   // (the tiles are loaded again)
+    {
+      const float scale2 = mask(j0 + 32 * subs - 32);
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sum += __builtin_amdgcn_exp2f(fmaf(s[i], scale2, SUM ? off[i] : -m));
+      finish(sum, scale2, (tiles - 1) % WG_BUFFERS, (subs - 1) & 1);
+    }
+    if (SUM) {
+      __syncthreads();
+      if (tiles > 1) add_tile(tiles - 2);
+      add_tile(tiles - 1);
+      __syncthreads();
+    }
   }
 
   if (SUM) {
     __syncthreads();
-    float* const to = P.supers > 1 ? P.part + ((size_t)g * P.supers + blockIdx.y) * P.T : P.out + (size_t)g * P.T;
-    for (int i = threadIdx.x; i < P.rows && j0 + i < P.T; i += 64 * WG_WAVES)
-      to[j0 + i] = sh_sum[i] + sh_sum[P.rows + i] + sh_sum[2 * P.rows + i] + sh_sum[3 * P.rows + i];
+    // nobody reads what a part has of keys behind the last that its columns see; in the result those weigh nothing
+    const int seen = max(min(jn, weigh_last_key(P, n, super, BLOCK) + 1) - j0, 0), all = P.supers > 1 ? seen : min(P.rows, P.T - j0);
+    for (int i = (P.per > 1 ? 0 : seen) + threadIdx.x; i < all; i += 64 * WAVES) to[j0 + i] = i < seen ? sh_sum[i] : 0.f;
     return;
   }
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    const int col = block0 * WG_BLOCK + wave * 64 + 32 * t + (lane & 31);
-    const float M = ri_xor_max<32>(m[t]);
-    const float Z = ri_xor_sum<32>(m[t] == -INFINITY ? l[t] : l[t] * __builtin_amdgcn_exp2f(m[t] - M));
-    if (lane < 32) {
-      float* const at = P.stats + (((size_t)g * P.S + blockIdx.z) * P.cols_pad + col) * 2;
-      at[0] = col < P.cols ? M : -INFINITY;
-      at[1] = col < P.cols ? Z : 0.f;
-    }
+  const float M = ri_xor_max<32>(m);
+  const float Z = ri_xor_sum<32>(m == -INFINITY ? l : l * __builtin_amdgcn_exp2f(m - M));
+  if (lane < 32) {
+    const int col = block0 * BLOCK + wave * 32 + lane;
+    float* const to = P.stats + (((size_t)g * P.S + blockIdx.z) * P.cols_pad + col) * 2;
+    to[0] = col < P.cols ? M : -INFINITY;
+    to[1] = col < P.cols ? Z : 0.f;
   }
 }
 
@@ -305,32 +324,47 @@ __global__ __launch_bounds__(256) void weigh_join_kernel(WeighParams P) {
   if ((threadIdx.x & 7) == 0) P.lse[(size_t)g * P.cols_pad + col] = lse;
 }
 
-// Grid (ceil(T / 256), B * heads): a thread adds the columns' blocks of a key.
+// Grid (ceil(T / 256), B * heads): a thread adds the parts of a key, of those that have columns that see it.
 __global__ __launch_bounds__(256) void weigh_add_kernel(WeighParams P) {
-  const int g = blockIdx.y, j = blockIdx.x * 256 + threadIdx.x;
+  const int g = blockIdx.y, j = blockIdx.x * 256 + threadIdx.x, n = weigh_len(P, g / P.heads);
   if (j >= P.T) return;
   float x = 0.f;
-  for (int s = 0; s < P.supers; ++s) x += P.part[((size_t)g * P.supers + s) * P.T + j];
+  if (j < n) {
+    const float* const from = P.part + (size_t)g * P.supers * P.T + j;
+    int s = max(j - (n - P.W), 0) * P.gs / (WG_SUM_COLS * P.per);
+    for (; s + 8 <= P.supers; s += 8) {
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = from[(size_t)(s + i) * P.T];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x += v[i];
+    }
+    for (; s < P.supers; ++s) x += from[(size_t)s * P.T];
+  }
   P.out[(size_t)g * P.T + j] = x;
 }
 
 // ------------------------------------------------------------------------------------ host side
 struct WeighPlan { int cols_pad, S, rows, per, supers; bool joined; };
 static int weigh_up(int64_t n, int to) { return (int)((n + to - 1) / to * to); }
+// Keys of a split: as many workgroups of the first pass as fit the compute units at a time, two to each, and no more keys than
+// the second has LDS for.  The second pass takes one block of columns to a workgroup, whose sums are a part of the result (8192
+// queries and keys, 32 heads: parts of 67 MB), and more of them, which it adds up in LDS, where the parts would pass 256 MB.
+// Two blocks over few keys are one workgroup's too (a launch less: 224 columns, 1111 keys, 4 heads 21.6 -> 17.4 us; up to 448 keys
+// LDS still holds three workgroups, of more it costs more than the launch).  Up to sixteen splits are joined by whoever needs them,
+// more by a launch of their own.
 static WeighPlan weigh_plan(int64_t groups, int cols, int T) {
   WeighPlan p;
-  p.cols_pad = weigh_up(cols, WG_BLOCK);
-  const int64_t blocks = p.cols_pad / WG_BLOCK;
-  // keys of a split: workgroups for the compute units, and no more keys than there is LDS for their sums
-  const int64_t want = (T * groups * blocks + 767) / 768;
+  p.cols_pad = weigh_up(cols, WG_COLS);
+  const int64_t want = (T * groups * (p.cols_pad / WG_COLS) + 511) / 512;
   p.rows = weigh_up(want < 128 ? 128 : want > WG_ROWS ? WG_ROWS : want, WG_TILE);
   p.S = (T + p.rows - 1) / p.rows;
-  // blocks of columns whose sums a workgroup of the second kernel adds up
-  p.per = (int)(groups * p.S * blocks / 2048);
-  if (p.per > 8) p.per = 8;
-  if (p.per < 1) p.per = 1;
+  const int64_t blocks = weigh_up(cols, WG_SUM_COLS) / WG_SUM_COLS;
+  const int64_t per = (groups * blocks * T * (int64_t)sizeof(float) + (1 << 28) - 1) >> 28;
+  p.per = (int)(per < blocks ? per : blocks);
+  if (blocks == 2 && p.rows <= 448) p.per = 2;
   p.supers = (int)((blocks + p.per - 1) / p.per);
-  p.joined = p.S > 8;
+  p.joined = p.S > 16;
   return p;
 }
 
@@ -342,10 +376,9 @@ extern "C" size_t ri_attention_weights_workspace_bytes(int B, int heads, int gs,
 
 template <int D, bool HALF>
 static void launch_weigh(const WeighParams& P, int groups, hipStream_t s) {
-  const int blocks = P.cols_pad / WG_BLOCK;
-  weigh_kernel<D, HALF, false><<<dim3(groups, blocks, P.S), 64 * WG_WAVES, 0, s>>>(P);
+  weigh_kernel<D, HALF, false, WG_COLS / 32, 4><<<dim3(groups, P.cols_pad / WG_COLS, P.S), 2 * WG_COLS, 0, s>>>(P);
   if (P.joined) weigh_join_kernel<<<dim3(P.cols_pad / 32, groups), 256, 0, s>>>(P);
-  weigh_kernel<D, HALF, true><<<dim3(groups, P.supers, P.S), 64 * WG_WAVES, WG_WAVES * P.rows * sizeof(float), s>>>(P);
+  weigh_kernel<D, HALF, true, WG_SUM_COLS / 32, 3><<<dim3(groups, P.supers, P.S), 2 * WG_SUM_COLS, P.per > 1 ? P.rows * sizeof(float) : 0, s>>>(P);
   if (P.supers > 1) weigh_add_kernel<<<dim3((P.T + 255) / 256, groups), 256, 0, s>>>(P);
 }
 

@@ -331,11 +331,14 @@ struct PagedAppendParams {
   int budget, sinks, recent, dim;
 };
 
-#define PG_APPEND_THREADS 512
+// four values to a row that need not be aligned to more than one
+typedef float pg_f4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef int pg_i4 __attribute__((ext_vector_type(4), aligned(4)));
 
-// Grid (heads, B).
-__global__ __launch_bounds__(PG_APPEND_THREADS) void paged_append_kernel(PagedAppendParams P) {
-  __shared__ unsigned long long sh_best[PG_APPEND_THREADS / 64];
+// Grid (heads, B).  The search for the weakest row reads eight bytes to a row, four rows to a lane's load and U loads ahead.
+template <int THREADS, int U>
+__global__ __launch_bounds__(THREADS) void paged_append_kernel(PagedAppendParams P) {
+  __shared__ unsigned long long sh_best[THREADS / 64];
   const int head = blockIdx.x, b = blockIdx.y;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int held = min(max(P.lens[b], 0), P.budget);
@@ -346,23 +349,47 @@ __global__ __launch_bounds__(PG_APPEND_THREADS) void paged_append_kernel(PagedAp
   int32_t* const positions = P.positions ? P.positions + b * P.pb + head * P.ph : nullptr;
   if (held == P.budget) {
     if (!scores) return;
-    unsigned long long best = ~0ull;
-    for (int r = threadIdx.x; r < held; r += PG_APPEND_THREADS) {
-      const int at = positions[r];
-      const bool stays = at < P.sinks || at > (int64_t)token - P.recent;
-      const unsigned long long mine = (unsigned long long)(stays ? 0xffffffffu : pg_order(scores[r])) << 32 | (uint32_t)r;
-      best = mine < best ? mine : best;
+    const int64_t old = (int64_t)token - P.recent;   // the last token that is not one of the recent ones
+    uint32_t best = 0xffffffffu;
+    int best_row = 0;
+    const auto take = [&](int r, float score, int at) {   // (rows ascend: the first of equal ones stays)
+      const uint32_t o = at < P.sinks || at > old ? 0xffffffffu : pg_order(score);
+      if (o < best) { best = o; best_row = r; }
+    };
+    int r0 = threadIdx.x * 4;
+    const int whole = held & ~3;
+    for (; r0 + (U - 1) * THREADS * 4 < whole; r0 += U * THREADS * 4) {
+      pg_f4 s[U];
+      pg_i4 at[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        s[u] = *reinterpret_cast<const pg_f4*>(scores + r0 + u * THREADS * 4);
+        at[u] = *reinterpret_cast<const pg_i4*>(positions + r0 + u * THREADS * 4);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) take(r0 + u * THREADS * 4 + i, s[u][i], at[u][i]);
     }
+    for (; r0 < whole; r0 += THREADS * 4) {
+      const pg_f4 s = *reinterpret_cast<const pg_f4*>(scores + r0);
+      const pg_i4 at = *reinterpret_cast<const pg_i4*>(positions + r0);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) take(r0 + i, s[i], at[i]);
+    }
+    if ((int)threadIdx.x < (held & 3)) take(whole + threadIdx.x, scores[whole + threadIdx.x], positions[whole + threadIdx.x]);
+    unsigned long long both = (unsigned long long)best << 32 | (uint32_t)best_row;
 #pragma unroll
     for (int d = 32; d; d >>= 1) {
-      const unsigned long long other = __shfl_xor(best, d);
-      best = other < best ? other : best;
+      const unsigned long long other = __shfl_xor(both, d);
+      both = other < both ? other : both;
     }
-    if (lane == 0) sh_best[wave] = best;
+    if (lane == 0) sh_best[wave] = both;
     __syncthreads();
-    best = sh_best[0];
-    for (int w = 1; w < PG_APPEND_THREADS / 64; ++w) best = sh_best[w] < best ? sh_best[w] : best;
-    row = (int)(uint32_t)best;
+    both = sh_best[0];
+#pragma unroll
+    for (int w = 1; w < THREADS / 64; ++w) both = sh_best[w] < both ? sh_best[w] : both;
+    row = (int)(uint32_t)both;
   }
   const int page = P.c.table[b * P.c.ts + (row >> P.c.shift)];
   if ((unsigned)page >= (unsigned)P.c.pages) return;
@@ -395,96 +422,278 @@ struct PagedFillParams {
   int32_t* positions;
   int64_t sb, sh, pb, ph;
   int32_t* kept;          // [B * heads, budget]: the kept rows in order
-  int T, budget, sinks, recent, dim;
+  // a selection over several chunks of a prompt
+  uint16_t* hist;         // [B * heads, chunks, 2048] rows of a chunk by the first digit of their order, and [.., 64] by its bits 10 .. 5
+  uint16_t* coarse;
+  uint32_t* tied;         // [B * heads, chunks * PG_CHUNK]: the orders of a chunk's rows that share the digit in question
+  int2* counts;           // [B * heads, chunks]: rows above that digit, rows of it; then where a chunk's rows go, ties in front
+  int2* limit;            // [B * heads]: the digit and how many of its rows are kept; then the lowest kept order and its rows
+  int T, budget, sinks, recent, dim, chunks;
 };
 
 __device__ __forceinline__ int pg_prompt(const PagedFillParams& P, int b) { return P.lens ? min(max(P.lens[b], 0), P.T) : P.T; }
 
 #define PG_SEL_THREADS 1024
+#define PG_SEL_WAVES (PG_SEL_THREADS / 64)
+#define PG_CHUNK (4 * PG_SEL_THREADS)   // rows of a workgroup: four consecutive ones to a thread
 
 // The rows of a prompt that are kept, in order, with their weights and positions: the `sinks` first, the `recent` last and of the
-// others those with the highest weights, at equal weights the first ones.  Grid (heads, B); a radix selection of the lowest kept
-// weight (digits of 11, 11 and 10 bits), then one pass that lists.
-__global__ __launch_bounds__(PG_SEL_THREADS) void paged_select_kernel(PagedFillParams P) {
-  constexpr int NW = PG_SEL_THREADS / 64;
-  __shared__ int hist[2048];
-  __shared__ int sh_scan[NW], sh_pick[2], sh_tot[2][NW];
-  const int head = blockIdx.x, b = blockIdx.y, n = pg_prompt(P, b);
+// others those with the highest weights, at equal weights the first ones.  A radix selection finds the lowest kept order, digits of
+// 11, 11 and 10 bits, and how many of the rows of that order are kept, the first ones.
+struct PagedRows {   // this thread's rows of a chunk
+  int r0;
+  uint32_t o[4];     // their orders; none is 0
+  float w[4];
+};
+__device__ __forceinline__ PagedRows pg_rows(const PagedFillParams& P, const float* w, int n, int chunk) {
+  PagedRows x;
+  x.r0 = chunk * PG_CHUNK + 4 * threadIdx.x;
+  if (x.r0 + 4 <= n) {
+    const pg_f4 v = *reinterpret_cast<const pg_f4*>(w + x.r0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x.w[i] = v[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x.w[i] = x.r0 + i < n ? w[x.r0 + i] : 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = x.r0 + i;
+    x.o[i] = r >= n ? 0u : r < P.sinks || r >= n - P.recent ? 0xffffffffu : pg_order(x.w[i]);
+  }
+  return x;
+}
+
+// Whole workgroup: the bin from the top of hist[bins] (LDS, 2048 at most) in which the count reaches need; need becomes how many of
+// that bin's are kept.
+__device__ __forceinline__ int pg_pick(const int* hist, int bins, int& need) {
+  __shared__ int sh_scan[PG_SEL_WAVES], sh_pick[2];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  __syncthreads();
+  const int top = bins - 1 - 2 * (int)threadIdx.x;   // thread t: bins 2 t and 2 t + 1 from the top
+  const int a = top >= 0 ? hist[top] : 0, c = top >= 1 ? hist[top - 1] : 0;
+  const int incl = (int)ri_wave_incl_scan((uint32_t)(a + c));
+  if (lane == 63) sh_scan[wave] = incl;
+  __syncthreads();
+  int before = incl - a - c;
+#pragma unroll
+  for (int i = 0; i < PG_SEL_WAVES; ++i) before += i < wave ? sh_scan[i] : 0;
+  if (before < need && before + a + c >= need) {
+    const bool second = before + a < need;
+    sh_pick[0] = second ? top - 1 : top;
+    sh_pick[1] = need - before - (second ? a : 0);
+  }
+  __syncthreads();
+  need = sh_pick[1];
+  return sh_pick[0];
+}
+
+// Whole workgroup: exclusive sums over the threads of a count below 2^16 in each half of x; the workgroup's in *all.
+__device__ __forceinline__ uint32_t pg_scan(uint32_t x, uint32_t* all) {
+  __shared__ uint32_t sh_wave[PG_SEL_WAVES];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint32_t incl = ri_wave_incl_scan(x);
+  __syncthreads();
+  if (lane == 63) sh_wave[wave] = incl;
+  __syncthreads();
+  uint32_t before = 0, total = 0;
+#pragma unroll
+  for (int i = 0; i < PG_SEL_WAVES; ++i) {
+    const uint32_t v = sh_wave[i];
+    before += i < wave ? v : 0;
+    total += v;
+  }
+  *all = total;
+  return before + incl - x;
+}
+
+// This thread's rows of order above `lowest`, and the first `need` of those of it, to their places: `base` rows and `ties` of that
+// order are in front of the chunk's.
+__device__ __forceinline__ void pg_emit(const PagedFillParams& P, int g, int b, int head, const PagedRows& x, uint32_t lowest, int need,
+                                        int base, int ties) {
+  uint32_t mine = 0, all;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) mine += (x.o[i] > lowest ? 1u : 0u) + (x.o[i] == lowest ? 0x10000u : 0u);
+  const uint32_t before = pg_scan(mine, &all);
+  int above = before & 0xffffu, tie = ties + (int)(before >> 16);
+  int32_t* const kept = P.kept + (size_t)g * P.budget;
+  float* const scores = P.scores ? P.scores + b * P.sb + head * P.sh : nullptr;
+  int32_t* const positions = P.positions ? P.positions + b * P.pb + head * P.ph : nullptr;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const bool is_above = x.o[i] > lowest, is_tie = x.o[i] == lowest;
+    if (is_above || (is_tie && tie < need)) {
+      const int at = base + above + min(tie, need) - min(ties, need);
+      kept[at] = x.r0 + i;
+      if (scores) scores[at] = x.w[i];
+      if (positions) positions[at] = x.r0 + i;
+    }
+    above += is_above;
+    tie += is_tie;
+  }
+}
+
+// Scores and positions of the rows [r0, r1) of a prompt that is kept whole.
+__device__ __forceinline__ void pg_whole(const PagedFillParams& P, int b, int head, int r0, int r1) {
   const float* const w = P.weights ? P.weights + b * P.wb + head * P.wh : nullptr;
   float* const scores = P.scores ? P.scores + b * P.sb + head * P.sh : nullptr;
   int32_t* const positions = P.positions ? P.positions + b * P.pb + head * P.ph : nullptr;
-  if (n <= P.budget) {
-    for (int r = threadIdx.x; r < n; r += PG_SEL_THREADS) {
-      if (scores) scores[r] = w[r];
-      if (positions) positions[r] = r;
-    }
-    return;
+  for (int r = r0 + threadIdx.x; r < r1; r += PG_SEL_THREADS) {
+    if (scores) scores[r] = w[r];
+    if (positions) positions[r] = r;
   }
-  const auto order_of = [&](int r) {
-    return r < P.sinks || r >= n - P.recent ? 0xffffffffu : pg_order(w[r]);
-  };
-  uint32_t prefix = 0, known = 0;   // bits of the lowest kept order found so far
-  int need = P.budget;              // of the rows whose bits agree, the highest `need` are kept
+}
+
+// Grid (heads, B): prompts of one chunk at most, and longer ones that are kept whole (ALL).
+template <bool ALL>
+__global__ __launch_bounds__(PG_SEL_THREADS) void paged_select_kernel(PagedFillParams P) {
+  __shared__ int hist[2048];
+  const int head = blockIdx.x, b = blockIdx.y, n = pg_prompt(P, b), g = b * P.c.heads + head;
+  if (n <= P.budget) return pg_whole(P, b, head, 0, n);
+  if (ALL) return;
+  const PagedRows x = pg_rows(P, P.weights + b * P.wb + head * P.wh, n, 0);
+  uint32_t lowest = 0, known = 0;   // bits of the lowest kept order found so far
+  int need = P.budget;
+#pragma unroll
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
-    for (int i = threadIdx.x; i < 2048; i += PG_SEL_THREADS) hist[i] = 0;
+    hist[threadIdx.x] = hist[threadIdx.x + PG_SEL_THREADS] = 0;
     __syncthreads();
-    for (int r = threadIdx.x; r < n; r += PG_SEL_THREADS) {
-      const uint32_t o = order_of(r);
-      if ((o & known) == prefix) atomicAdd(&hist[(o >> shift) & (bins - 1)], 1);
-    }
-    __syncthreads();
-    // the bin from the top in which the count reaches `need`: thread t has bins 2 t and 2 t + 1 from the top
-    const int top = bins - 1 - 2 * (int)threadIdx.x;
-    const int a = top >= 0 ? hist[top] : 0, c = top >= 1 ? hist[top - 1] : 0;
-    const int incl = (int)ri_wave_incl_scan((uint32_t)(a + c));
-    if (lane == 63) sh_scan[wave] = incl;
-    __syncthreads();
-    int before = incl - a - c;
-    for (int i = 0; i < wave; ++i) before += sh_scan[i];
-    if (before < need && before + a + c >= need) {
-      const bool second = before + a < need;
-      sh_pick[0] = second ? top - 1 : top;
-      sh_pick[1] = need - before - (second ? a : 0);
-    }
-    __syncthreads();
-    prefix |= (uint32_t)sh_pick[0] << shift;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (x.o[i] && (x.o[i] & known) == lowest) atomicAdd(&hist[(x.o[i] >> shift) & (bins - 1)], 1);
+    lowest |= (uint32_t)pg_pick(hist, bins, need) << shift;
     known |= (uint32_t)(bins - 1) << shift;
-    need = sh_pick[1];
     __syncthreads();
   }
-  // rows above the found order are kept, and the first `need` of those at it
-  int32_t* const kept = P.kept + ((size_t)b * P.c.heads + head) * P.budget;
+  pg_emit(P, g, b, head, x, lowest, need, 0, 0);
+}
+
+// Longer prompts: four launches over all chunks, one of them over the rows in question only.  1: the chunks' rows by the first
+// digit.  Grid (chunks, heads, B).
+__global__ __launch_bounds__(PG_SEL_THREADS) void paged_digit_kernel(PagedFillParams P) {
+  __shared__ int hist[2048];
+  const int chunk = blockIdx.x, head = blockIdx.y, b = blockIdx.z, n = pg_prompt(P, b);
+  if (n <= P.budget || chunk * PG_CHUNK >= n) return;
+  const PagedRows x = pg_rows(P, P.weights + b * P.wb + head * P.wh, n, chunk);
+  hist[threadIdx.x] = hist[threadIdx.x + PG_SEL_THREADS] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (x.o[i]) atomicAdd(&hist[x.o[i] >> 21], 1);
+  __syncthreads();
+  const size_t at = (size_t)(b * P.c.heads + head) * P.chunks + chunk;
+  const int lo = hist[2 * threadIdx.x], hi = hist[2 * threadIdx.x + 1];
+  reinterpret_cast<uint32_t*>(P.hist + at * 2048)[threadIdx.x] = (uint32_t)lo | (uint32_t)hi << 16;   // (4096 at most)
+  float sum = (float)(lo + hi);   // of 32 bins, sixteen lanes
+  sum = ri_xor_sum<1>(ri_xor_sum<2>(ri_xor_sum<4>(ri_xor_sum<8>(sum))));
+  if (threadIdx.x % 16 == 0) P.coarse[at * 64 + threadIdx.x / 16] = (uint16_t)sum;
+}
+
+// 2: the digit in which the count of kept rows ends, and of a chunk how many rows are above it and the orders of those that have it.
+// Grid (chunks, heads, B).
+__global__ __launch_bounds__(PG_SEL_THREADS) void paged_tied_kernel(PagedFillParams P) {
+  __shared__ int hist[64];
+  const int chunk = blockIdx.x, head = blockIdx.y, b = blockIdx.z, n = pg_prompt(P, b), g = b * P.c.heads + head;
+  if (n <= P.budget || chunk * PG_CHUNK >= n) return;
+  const PagedRows x = pg_rows(P, P.weights + b * P.wb + head * P.wh, n, chunk);
+  const int chunks = (n + PG_CHUNK - 1) / PG_CHUNK, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int need = P.budget, digit = 0;
+#pragma unroll
+  for (int fine = 0; fine < 2; ++fine) {   // 64 groups of 32 digits, then the digits of one
+    if (threadIdx.x < 64) hist[threadIdx.x] = 0;
+    __syncthreads();
+    int sum = 0;
+    if (!fine || lane < 32) {
+#pragma unroll 4
+      for (int c = wave; c < chunks; c += PG_SEL_WAVES) {
+        const size_t at = (size_t)g * P.chunks + c;
+        sum += fine ? P.hist[at * 2048 + digit * 32 + lane] : P.coarse[at * 64 + lane];
+      }
+      if (sum) atomicAdd(&hist[lane], sum);
+    }
+    digit = digit * 32 + pg_pick(hist, fine ? 32 : 64, need);
+    __syncthreads();
+  }
+  uint32_t mine = 0, all;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    mine += (x.o[i] && (int)(x.o[i] >> 21) > digit ? 1u : 0u) + (x.o[i] && (int)(x.o[i] >> 21) == digit ? 0x10000u : 0u);
+  uint32_t* to = P.tied + ((size_t)g * P.chunks + chunk) * PG_CHUNK + (pg_scan(mine, &all) >> 16);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (x.o[i] && (int)(x.o[i] >> 21) == digit) *to++ = x.o[i];
+  if (threadIdx.x == 0) {
+    P.counts[(size_t)g * P.chunks + chunk] = make_int2(all & 0xffffu, all >> 16);
+    if (chunk == 0) P.limit[g] = make_int2(digit, need);
+  }
+}
+
+// 3: the lowest kept order and where each chunk's rows go.  Grid (heads, B); a wave takes a chunk's tied rows at a time.
+__global__ __launch_bounds__(PG_SEL_THREADS) void paged_limit_kernel(PagedFillParams P) {
+  __shared__ int hist[2048];
+  __shared__ uint32_t sh_chunk[PG_SEL_THREADS];
+  const int head = blockIdx.x, b = blockIdx.y, n = pg_prompt(P, b), g = b * P.c.heads + head;
+  if (n <= P.budget) return;
+  const int chunks = (n + PG_CHUNK - 1) / PG_CHUNK, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int2* const counts = P.counts + (size_t)g * P.chunks;
+  const uint32_t* const tied = P.tied + (size_t)g * P.chunks * PG_CHUNK;
+  int need = P.limit[g].y;
+  uint32_t lowest = (uint32_t)P.limit[g].x << 21, known = 0x7ffu << 21;
+#pragma unroll
+  for (int pass = 1; pass < 3; ++pass) {
+    const int shift = pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
+    hist[threadIdx.x] = hist[threadIdx.x + PG_SEL_THREADS] = 0;
+    __syncthreads();
+    for (int c = wave; c < chunks; c += PG_SEL_WAVES) {
+      const int m = counts[c].y;
+      for (int i = lane; i < m; i += 64) {
+        const uint32_t o = tied[(size_t)c * PG_CHUNK + i];
+        if ((o & known) == lowest) atomicAdd(&hist[(o >> shift) & (bins - 1)], 1);
+      }
+    }
+    lowest |= (uint32_t)pg_pick(hist, bins, need) << shift;
+    known |= (uint32_t)(bins - 1) << shift;
+    __syncthreads();
+  }
   int base = 0, ties = 0;
-  for (int r0 = 0; r0 < n; r0 += PG_SEL_THREADS) {
-    const int r = r0 + threadIdx.x;
-    const uint32_t o = r < n ? order_of(r) : 0u;
-    const bool above = r < n && o > prefix, equal = r < n && o == prefix;
-    const uint64_t ma = __ballot(above), me = __ballot(equal), below = (1ull << lane) - 1;
-    if (lane == 0) {
-      sh_tot[0][wave] = __popcll(ma);
-      sh_tot[1][wave] = __popcll(me);
+  for (int c0 = 0; c0 < chunks; c0 += PG_SEL_THREADS) {
+    const int c1 = min(chunks, c0 + PG_SEL_THREADS);
+    for (int c = c0 + wave; c < c1; c += PG_SEL_WAVES) {
+      const int m = counts[c].y;
+      int above = 0, equal = 0;
+      for (int i = lane; i < m; i += 64) {
+        const uint32_t o = tied[(size_t)c * PG_CHUNK + i];
+        above += o > lowest;
+        equal += o == lowest;
+      }
+      const uint32_t sum = __shfl(ri_wave_incl_scan((uint32_t)above | (uint32_t)equal << 16), 63);
+      if (lane == 0) sh_chunk[c - c0] = sum;
     }
     __syncthreads();
-    int na = 0, ne = 0, ta = 0, te = 0;
-    for (int i = 0; i < NW; ++i) {
-      if (i < wave) { na += sh_tot[0][i]; ne += sh_tot[1][i]; }
-      ta += sh_tot[0][i];
-      te += sh_tot[1][i];
-    }
-    na += __popcll(ma & below);
-    ne += __popcll(me & below) + ties;       // ties in front of this row
-    const int at = base + na + min(ne, need) - min(ties, need);
-    if (above || (equal && ne < need)) {
-      kept[at] = r;
-      if (scores) scores[at] = w[r];
-      if (positions) positions[at] = r;
-    }
-    base += ta + min(ties + te, need) - min(ties, need);
-    ties += te;
+    const int c = c0 + threadIdx.x;
+    const int above = c < c1 ? counts[c].x + (int)(sh_chunk[threadIdx.x] & 0xffffu) : 0;
+    const int equal = c < c1 ? (int)(sh_chunk[threadIdx.x] >> 16) : 0;
+    // (a chunk has 4096 rows and a part of 1024 chunks 2^22: sums of their own)
+    uint32_t all_above, all_equal;
+    const int b0 = base + (int)pg_scan((uint32_t)above, &all_above);
+    const int t0 = ties + (int)pg_scan((uint32_t)equal, &all_equal);
+    if (c < c1) counts[c] = make_int2(b0 + min(t0, need), t0);
+    base += (int)all_above;
+    ties += (int)all_equal;
     __syncthreads();
   }
+  if (threadIdx.x == 0) P.limit[g] = make_int2((int)lowest, need);
+}
+
+// 4: the list.  Grid (chunks, heads, B).
+__global__ __launch_bounds__(PG_SEL_THREADS) void paged_list_kernel(PagedFillParams P) {
+  const int chunk = blockIdx.x, head = blockIdx.y, b = blockIdx.z, n = pg_prompt(P, b), g = b * P.c.heads + head;
+  if (chunk * PG_CHUNK >= n) return;
+  if (n <= P.budget) return pg_whole(P, b, head, chunk * PG_CHUNK, min(n, (chunk + 1) * PG_CHUNK));
+  const PagedRows x = pg_rows(P, P.weights + b * P.wb + head * P.wh, n, chunk);
+  const int2 limit = P.limit[g], at = P.counts[(size_t)g * P.chunks + chunk];
+  pg_emit(P, g, b, head, x, (uint32_t)limit.x, limit.y, at.x, at.y);
 }
 
 // Grid (ceil(rows / rows per workgroup), heads, B): the kept rows into their pages, a row by dim / 8 lanes.
@@ -612,13 +821,42 @@ extern "C" int ri_paged_append(const ri_paged_t* cache, const void* key, const v
   P.sb = score_batch_stride; P.sh = score_head_stride; P.pb = position_batch_stride; P.ph = position_head_stride;
   P.token = token_positions;
   P.budget = budget; P.sinks = sinks; P.recent = recent; P.dim = cache->dim;
-  paged_append_kernel<<<dim3(cache->heads, B), PG_APPEND_THREADS, 0, (hipStream_t)stream>>>(P);
+  const dim3 grid(cache->heads, B);
+  if (!scores || budget <= 2048) paged_append_kernel<256, 2><<<grid, 256, 0, (hipStream_t)stream>>>(P);
+  else paged_append_kernel<1024, 2><<<grid, 1024, 0, (hipStream_t)stream>>>(P);
   RI_HIP_CHECK_LAUNCH();
   return RI_OK;
 }
 
+// 16-byte aligned parts of the workspace of a fill: kept, hist, coarse, tied, counts, limit
+static size_t paged_fill_carve(PagedFillParams* P, size_t groups, int T, int budget, char* at) {
+  const size_t chunks = T > PG_CHUNK ? ((size_t)T + PG_CHUNK - 1) / PG_CHUNK : 0;
+  size_t used = 0;
+  const auto part = [&](size_t bytes) {
+    char* const p = at + used;
+    used += (bytes + 15) / 16 * 16;
+    return p;
+  };
+  char* const kept = part(groups * budget * 4);
+  char* const hist = part(groups * chunks * 2048 * 2);
+  char* const coarse = part(groups * chunks * 64 * 2);
+  char* const tied = part(groups * chunks * PG_CHUNK * 4);
+  char* const counts = part(groups * chunks * sizeof(int2));
+  char* const limit = part(groups * sizeof(int2));
+  if (P) {
+    P->kept = (int32_t*)kept;
+    P->hist = (uint16_t*)hist;
+    P->coarse = (uint16_t*)coarse;
+    P->tied = (uint32_t*)tied;
+    P->counts = (int2*)counts;
+    P->limit = (int2*)limit;
+    P->chunks = (int)chunks;
+  }
+  return used;
+}
+
 extern "C" size_t ri_paged_fill_workspace_bytes(int B, int heads, int T, int budget) {
-  return B <= 0 || heads <= 0 || T <= budget || budget <= 0 ? 0 : (size_t)B * heads * budget * sizeof(int32_t);
+  return B <= 0 || heads <= 0 || T <= budget || budget <= 0 ? 0 : paged_fill_carve(nullptr, (size_t)B * heads, T, budget, nullptr);
 }
 
 extern "C" int ri_paged_fill(const ri_paged_t* cache, const void* key, const void* value, int64_t key_batch_stride,
@@ -653,10 +891,20 @@ extern "C" int ri_paged_fill(const ri_paged_t* cache, const void* key, const voi
   P.scores = scores;
   P.positions = positions;
   P.sb = score_batch_stride; P.sh = score_head_stride; P.pb = position_batch_stride; P.ph = position_head_stride;
-  P.kept = (int32_t*)workspace;
+  if (need) paged_fill_carve(&P, (size_t)B * cache->heads, T, budget, (char*)workspace);
   P.T = T; P.budget = budget; P.sinks = sinks; P.recent = recent; P.dim = cache->dim;
   hipStream_t s = (hipStream_t)stream;
-  if (T > budget || scores || positions) paged_select_kernel<<<dim3(cache->heads, B), PG_SEL_THREADS, 0, s>>>(P);
+  const dim3 each(cache->heads, B), chunks(P.chunks, cache->heads, B);
+  if (T <= budget) {
+    if (scores || positions) paged_select_kernel<true><<<each, PG_SEL_THREADS, 0, s>>>(P);
+  } else if (P.chunks == 0) {
+    paged_select_kernel<false><<<each, PG_SEL_THREADS, 0, s>>>(P);
+  } else {
+    paged_digit_kernel<<<chunks, PG_SEL_THREADS, 0, s>>>(P);
+    paged_tied_kernel<<<chunks, PG_SEL_THREADS, 0, s>>>(P);
+    paged_limit_kernel<<<each, PG_SEL_THREADS, 0, s>>>(P);
+    paged_list_kernel<<<chunks, PG_SEL_THREADS, 0, s>>>(P);
+  }
   const int per = 256 / (cache->dim / 8);
   paged_copy_kernel<<<dim3((room + per - 1) / per, cache->heads, B), 256, 0, s>>>(P);
   RI_HIP_CHECK_LAUNCH();

@@ -14,6 +14,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <cmath>
 #include <vector>
 
 #include "../../include/retro_mi355.h"
@@ -287,6 +288,14 @@ PyObject* gather_vectors(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+PyObject* pair_of(at::Tensor&& out, at::Tensor&& lse) {
+  PyObject *a = THPVariable_Wrap(std::move(out)), *b = THPVariable_Wrap(std::move(lse));
+  PyObject* both = a && b ? PyTuple_Pack(2, a, b) : nullptr;
+  Py_XDECREF(a);
+  Py_XDECREF(b);
+  return both;
+}
+
 // flash(q, k, v, weight, previous_out, previous_lse, cache_seqlens, workspace, scale, return_lse): the output, or (output, lse);
 // a status that is not zero; None as above.  q [BG, 1, gs, 128], k [BG, S, 1, 128]; the others by their elements.
 PyObject* flash(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -322,11 +331,241 @@ PyObject* flash(PyObject*, PyObject* const* args, Py_ssize_t n) {
   Py_END_ALLOW_THREADS
   if (status) return PyLong_FromLong(status);
   if (!with_lse) return THPVariable_Wrap(std::move(out));
-  PyObject *a = THPVariable_Wrap(std::move(out)), *b = THPVariable_Wrap(std::move(lse));
-  PyObject* both = a && b ? PyTuple_Pack(2, a, b) : nullptr;
-  Py_XDECREF(a);
-  Py_XDECREF(b);
-  return both;
+  return pair_of(std::move(out), std::move(lse));
+  END_HANDLE_TH_ERRORS
+}
+
+// ---- the paged cache's calls: arguments as the wrappers in kernels.py take them, checked as they check them (there the errors
+// are worded); anything that is not in order, and calls on another device than the current one, are left to them.
+
+// a plain tensor on `device` (null and true for None where it may be), of `dims` dimensions and `dtype`
+bool paged_tensor(PyObject* o, int dims, at::ScalarType dtype, int device, const at::Tensor** out, bool optional = false) {
+  *out = nullptr;
+  if (o == Py_None) return optional;
+  const at::Tensor* t = plain(o);
+  if (!t || !t->is_cuda() || t->get_device() != device || t->dim() != dims || t->scalar_type() != dtype) return false;
+  *out = t;
+  return true;
+}
+// strides of the dimensions in front of rows that are moved 16 bytes at a time (0 for one element)
+bool paged_rows(const at::Tensor& t, bool writes, int64_t* strides) {
+  const int64_t last = t.dim() - 1;
+  if (t.stride(last) != 1 || (uintptr_t)t.data_ptr() % 16) return false;
+  for (int64_t i = 0; i < last; ++i) {
+    strides[i] = t.size(i) > 1 ? t.stride(i) : 0;
+    if (strides[i] < 0 || strides[i] % 8 || (writes && t.size(i) > 1 && strides[i] == 0)) return false;
+  }
+  return true;
+}
+bool paged_pages(PyObject* const* args, int64_t B, bool writes, ri_paged_t* c, at::ScalarType* dtype, int* device) {
+  const at::Tensor *k = plain(args[0]), *v, *table;
+  if (!k || !k->is_cuda() || k->dim() != 4 || !half_type(k, *dtype)) return false;
+  *device = k->get_device();
+  if (*device != c10::hip::current_device() || !paged_tensor(args[1], 4, *dtype, *device, &v) ||
+      !paged_tensor(args[2], 2, at::kInt, *device, &table) || v->sizes() != k->sizes() || table->size(0) != B)
+    return false;
+  int64_t ks[3], vs[3];
+  const int64_t pages = k->size(0), heads = k->size(1), rows = k->size(2), dim = k->size(3), n = table->size(1);
+  if (pages < 1 || pages > INT32_MAX || heads < 1 || heads > 65535 || rows < 1 || rows & (rows - 1) || (dim != 64 && dim != 128) ||
+      !paged_rows(*k, writes, ks) || !paged_rows(*v, writes, vs) || n < 1 || n > (1 << 24) / rows || (n > 1 && table->stride(1) != 1) ||
+      table->stride(0) < 0)
+    return false;
+  *c = {k->data_ptr(), v->data_ptr(), (const int32_t*)table->data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], table->stride(0),
+        (int)pages, (int)heads, (int)rows, (int)dim, (int)n, *dtype == at::kHalf};
+  return true;
+}
+// one int32 to a sequence
+bool paged_each(PyObject* o, int64_t B, int device, const at::Tensor** out, bool optional = true) {
+  if (!paged_tensor(o, 1, at::kInt, device, out, optional)) return false;
+  return !*out || ((*out)->size(0) == B && (B == 1 || (*out)->stride(0) == 1));
+}
+// a value to each row, [B, heads, rows or more]; strides by sequence and head
+bool paged_values(PyObject* o, at::ScalarType dtype, int64_t B, int64_t heads, int64_t rows, int device, bool writes,
+                  const at::Tensor** out, int64_t* strides) {
+  strides[0] = strides[1] = 0;
+  if (!paged_tensor(o, 3, dtype, device, out, true)) return false;
+  const at::Tensor* t = *out;
+  if (!t) return true;
+  if (t->size(0) != B || t->size(1) != heads || t->size(2) < rows || (t->size(2) > 1 && t->stride(2) != 1)) return false;
+  const int64_t sb = B > 1 ? t->stride(0) : 0, sh = heads > 1 ? t->stride(1) : t->size(2);
+  if (sh < rows || (B > 1 && sb < rows) || (writes && B > 1 && heads > 1 && !(sb >= (heads - 1) * sh + rows || sh >= (B - 1) * sb + rows)))
+    return false;
+  strides[0] = sb;
+  strides[1] = sh;
+  return true;
+}
+// the scratch tensor, null where it is missing, elsewhere or too small
+void* paged_scratch(PyObject* o, size_t bytes, int device) {
+  const at::Tensor* t = plain(o);
+  return t && t->is_cuda() && t->get_device() == device && t->scalar_type() == at::kByte && t->is_contiguous() &&
+                 (size_t)t->numel() >= bytes ? t->data_ptr() : nullptr;
+}
+bool paged_scale(PyObject* o, int64_t dim, float* scale) {
+  if (o == Py_None) *scale = (float)(1.0 / sqrt((double)dim));
+  else if (PyFloat_CheckExact(o)) *scale = (float)PyFloat_AS_DOUBLE(o);
+  else return false;
+  return true;
+}
+// an int or, for None, `none`
+bool paged_int(PyObject* o, int64_t none, int64_t* out) {
+  if (o == Py_None) {
+    *out = none;
+    return true;
+  }
+  return PyLong_CheckExact(o) && integers(&o, 1, out);
+}
+
+// paged_attention(q, k_pages, v_pages, block_table, cache_seqlens, starts, scores, scale, return_lse, max_len, workspace)
+PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const at::Tensor *q, *lens, *starts, *scores;
+  ri_paged_t cache;
+  at::ScalarType dtype;
+  int device;
+  int64_t strides[2], max_len;
+  float scale;
+  if (n != 11 || at::impl::torch_function_mode_enabled()) Py_RETURN_NONE;
+  const at::Tensor* first = plain(args[0]);
+  if (!first || first->dim() != 4 || first->size(0) < 1 || first->size(0) > 65535 || first->size(1) != 1) Py_RETURN_NONE;
+  const int64_t B = first->size(0);
+  if (!paged_pages(args + 1, B, false, &cache, &dtype, &device) || !paged_tensor(args[0], 4, dtype, device, &q) ||
+      !q->is_contiguous() || (uintptr_t)q->data_ptr() % 16 || q->size(3) != cache.dim || q->size(2) % cache.heads)
+    Py_RETURN_NONE;
+  const int64_t hq = q->size(2), gs = hq / cache.heads, room = (int64_t)cache.table_pages * cache.page_rows;
+  if (gs < 1 || gs > 16 || !paged_each(args[4], B, device, &lens, false) || !paged_each(args[5], B, device, &starts) ||
+      !paged_int(args[9], room, &max_len) || max_len < 1 || max_len > room || !paged_scale(args[7], cache.dim, &scale) ||
+      !paged_values(args[6], at::kFloat, B, cache.heads, max_len, device, true, &scores, strides))
+    Py_RETURN_NONE;
+  const size_t bytes = ri_paged_attention_workspace_bytes((int)B, cache.heads, (int)gs, cache.dim, (int)max_len, scores != nullptr);
+  void* const ws = paged_scratch(args[10], bytes, device);
+  if (!ws || (args[8] != Py_True && args[8] != Py_False)) Py_RETURN_NONE;
+  const bool with_lse = args[8] == Py_True;
+  at::Tensor out = at::empty_like(*q), lse;
+  if (with_lse) lse = at::empty({B, hq}, q->options().dtype(at::kFloat).requires_grad(false));
+  void *qp = q->data_ptr(), *op = out.data_ptr(), *lp = with_lse ? lse.data_ptr() : nullptr;
+  void *np = address(lens), *sp = address(starts), *cp = address(scores);
+  const ri_stream_t stream = current_stream();
+  int status;
+  Py_BEGIN_ALLOW_THREADS
+  status = ri_paged_attention(&cache, qp, (const int32_t*)np, (const int32_t*)sp, (float*)cp, strides[0], strides[1], op, (float*)lp,
+                              (int)B, (int)gs, (int)max_len, scale, ws, bytes, stream);
+  Py_END_ALLOW_THREADS
+  if (status) return PyLong_FromLong(status);
+  return with_lse ? pair_of(std::move(out), std::move(lse)) : THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// paged_append(key, value, k_pages, v_pages, block_table, cache_seqlens, new_seqlens, scores, positions, token_positions, budget,
+// sinks, recent): status
+PyObject* paged_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const at::Tensor *key, *value, *lens, *held, *scores, *positions, *token;
+  ri_paged_t cache;
+  at::ScalarType dtype;
+  int device;
+  int64_t ks[3], vs[3], ss[2], ps[2], budget, sinks, recent;
+  if (n != 13 || !(key = plain(args[0])) || key->dim() != 4 || key->size(0) < 1 || key->size(0) > 65535 || key->size(1) != 1) Py_RETURN_NONE;
+  const int64_t B = key->size(0);
+  if (!paged_pages(args + 2, B, true, &cache, &dtype, &device) || !paged_tensor(args[0], 4, dtype, device, &key) ||
+      !paged_tensor(args[1], 4, dtype, device, &value) || key->size(2) != cache.heads || key->size(3) != cache.dim ||
+      value->sizes() != key->sizes() || !paged_rows(*key, false, ks) || !paged_rows(*value, false, vs))
+    Py_RETURN_NONE;
+  const int64_t room = (int64_t)cache.table_pages * cache.page_rows;
+  if (!paged_int(args[10], room, &budget) || !integers(args + 11, 1, &sinks) || !integers(args + 12, 1, &recent) || budget < 1 ||
+      budget > room || sinks + recent >= budget || !paged_each(args[5], B, device, &lens, false) ||
+      !paged_each(args[6], B, device, &held) || (held && held->data_ptr() == lens->data_ptr()) ||
+      !paged_values(args[7], at::kFloat, B, cache.heads, budget, device, true, &scores, ss) ||
+      !paged_values(args[8], at::kInt, B, cache.heads, budget, device, true, &positions, ps) ||
+      !paged_each(args[9], B, device, &token) || (scores && !positions) || (positions && !token))
+    Py_RETURN_NONE;
+  void *kp = key->data_ptr(), *vp = value->data_ptr(), *np = lens->data_ptr(), *hp = address(held), *sp = address(scores),
+       *pp = address(positions), *tp = address(token);
+  const ri_stream_t stream = current_stream();
+  int status;
+  Py_BEGIN_ALLOW_THREADS
+  status = ri_paged_append(&cache, kp, vp, ks[0], ks[2], vs[0], vs[2], (const int32_t*)np, (int32_t*)hp, (float*)sp, ss[0], ss[1],
+                           (int32_t*)pp, ps[0], ps[1], (const int32_t*)tp, (int)B, (int)budget, (int)sinks, (int)recent, stream);
+  Py_END_ALLOW_THREADS
+  return PyLong_FromLong(status);
+  END_HANDLE_TH_ERRORS
+}
+
+// paged_fill(key, value, k_pages, v_pages, block_table, new_seqlens, seqlens, weights, scores, positions, budget, sinks, recent,
+// workspace): status
+PyObject* paged_fill(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const at::Tensor *key, *value, *held, *lens, *weights, *scores, *positions;
+  ri_paged_t cache;
+  at::ScalarType dtype;
+  int device;
+  int64_t ks[3], vs[3], ws[2], ss[2], ps[2], budget, sinks, recent;
+  if (n != 14 || !(key = plain(args[0])) || key->dim() != 4 || key->size(0) < 1 || key->size(0) > 65535 || key->size(1) < 1 ||
+      key->size(1) > 1 << 24)
+    Py_RETURN_NONE;
+  const int64_t B = key->size(0), T = key->size(1);
+  if (!paged_pages(args + 2, B, true, &cache, &dtype, &device) || !paged_tensor(args[0], 4, dtype, device, &key) ||
+      !paged_tensor(args[1], 4, dtype, device, &value) || key->size(2) != cache.heads || key->size(3) != cache.dim ||
+      value->sizes() != key->sizes() || !paged_rows(*key, false, ks) || !paged_rows(*value, false, vs))
+    Py_RETURN_NONE;
+  const int64_t room = (int64_t)cache.table_pages * cache.page_rows;
+  if (!paged_int(args[10], room, &budget) || !integers(args + 11, 1, &sinks) || !integers(args + 12, 1, &recent) || budget < 1 ||
+      budget > room || sinks + recent > budget)
+    Py_RETURN_NONE;
+  const int64_t rows = T < budget ? T : budget;
+  if (!paged_each(args[5], B, device, &held) || !paged_each(args[6], B, device, &lens) ||
+      (held && lens && held->data_ptr() == lens->data_ptr()) ||
+      !paged_values(args[7], at::kFloat, B, cache.heads, T, device, false, &weights, ws) ||
+      !paged_values(args[8], at::kFloat, B, cache.heads, rows, device, true, &scores, ss) ||
+      !paged_values(args[9], at::kInt, B, cache.heads, rows, device, true, &positions, ps) || (!weights && (T > budget || scores)))
+    Py_RETURN_NONE;
+  const size_t bytes = ri_paged_fill_workspace_bytes((int)B, cache.heads, (int)T, (int)budget);
+  void* const work = bytes ? paged_scratch(args[13], bytes, device) : nullptr;
+  if (bytes && !work) Py_RETURN_NONE;
+  void *kp = key->data_ptr(), *vp = value->data_ptr(), *np = address(lens), *hp = address(held), *wp = address(weights),
+       *sp = address(scores), *pp = address(positions);
+  const ri_stream_t stream = current_stream();
+  int status;
+  Py_BEGIN_ALLOW_THREADS
+  status = ri_paged_fill(&cache, kp, vp, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], (const int32_t*)np, (const float*)wp, ws[0], ws[1],
+                         (int32_t*)hp, (float*)sp, ss[0], ss[1], (int32_t*)pp, ps[0], ps[1], (int)B, (int)T, (int)budget, (int)sinks,
+                         (int)recent, work, bytes, stream);
+  Py_END_ALLOW_THREADS
+  return PyLong_FromLong(status);
+  END_HANDLE_TH_ERRORS
+}
+
+// attention_weights(q, key, seqlens, scale, workspace): the weights, or a status that is not zero
+PyObject* attention_weights(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const at::Tensor *q, *key, *lens;
+  at::ScalarType dtype;
+  int64_t qs[3], ks[3];
+  float scale;
+  if (n != 5 || at::impl::torch_function_mode_enabled() || !(key = plain(args[1])) || !key->is_cuda() || key->dim() != 4 ||
+      !half_type(key, dtype))
+    Py_RETURN_NONE;
+  const int device = key->get_device();
+  if (device != c10::hip::current_device() || !paged_tensor(args[0], 4, dtype, device, &q)) Py_RETURN_NONE;
+  const int64_t B = q->size(0), W = q->size(1), hq = q->size(2), dim = q->size(3), T = key->size(1), heads = key->size(2);
+  if (B < 1 || heads < 1 || B > 65535 / heads || key->size(0) != B || key->size(3) != dim || (dim != 64 && dim != 128) || W < 1 ||
+      W > T || T > 1 << 24 || hq % heads || hq / heads < 1 || hq / heads > 16 || !paged_rows(*q, false, qs) ||
+      !paged_rows(*key, false, ks) || ks[1] > 1 << 23 || !paged_each(args[2], B, device, &lens) || !paged_scale(args[3], dim, &scale))
+    Py_RETURN_NONE;
+  const int gs = (int)(hq / heads);
+  const size_t bytes = ri_attention_weights_workspace_bytes((int)B, (int)heads, gs, (int)W, (int)T);
+  void* const ws = paged_scratch(args[4], bytes, device);
+  if (!ws) Py_RETURN_NONE;
+  at::Tensor out = at::empty({B, heads, T}, key->options().dtype(at::kFloat).requires_grad(false));
+  void *qp = q->data_ptr(), *kp = key->data_ptr(), *np = address(lens), *op = out.data_ptr();
+  const ri_stream_t stream = current_stream();
+  auto* call = dtype == at::kHalf ? ri_attention_weights_f16 : ri_attention_weights;
+  int status;
+  Py_BEGIN_ALLOW_THREADS
+  status = call(qp, kp, (const int32_t*)np, (float*)op, qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], (int)B, (int)W, (int)T, (int)heads,
+                gs, (int)dim, scale, ws, bytes, stream);
+  Py_END_ALLOW_THREADS
+  if (status) return PyLong_FromLong(status);
+  return THPVariable_Wrap(std::move(out));
   END_HANDLE_TH_ERRORS
 }
 
@@ -342,6 +581,10 @@ PyMethodDef methods[] = {{"append", (PyCFunction)(void (*)(void))append, METH_FA
                          {"gemm_softmax", (PyCFunction)(void (*)(void))gemm_softmax, METH_FASTCALL, nullptr},
                          {"gather_vectors", (PyCFunction)(void (*)(void))gather_vectors, METH_FASTCALL, nullptr},
                          {"flash", (PyCFunction)(void (*)(void))flash, METH_FASTCALL, nullptr},
+                         {"paged_attention", (PyCFunction)(void (*)(void))paged_attention, METH_FASTCALL, nullptr},
+                         {"paged_append", (PyCFunction)(void (*)(void))paged_append, METH_FASTCALL, nullptr},
+                         {"paged_fill", (PyCFunction)(void (*)(void))paged_fill, METH_FASTCALL, nullptr},
+                         {"attention_weights", (PyCFunction)(void (*)(void))attention_weights, METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_step_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

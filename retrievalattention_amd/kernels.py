@@ -819,6 +819,11 @@ def _on(device):
     return contextlib.nullcontext() if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
+def _held(t, tag, scratch):
+    """The scratch area `tag` as it is, for the native calls, which look whether it is large enough; None where there is none."""
+    return (shared_scratch if scratch is None else scratch).areas.get((getattr(t, "device", None), tag))
+
+
 def _strided(t, dims, dtype, device, name, writes=False):
     """Strides of all but the last dimension of a tensor whose rows are read or written 16 bytes at a time (of dimensions of one
     element: 0)."""
@@ -902,6 +907,10 @@ def paged_attention(q, k_pages, v_pages, block_table, cache_seqlens, starts=None
     max_len: no sequence has more rows (default: what the table holds; rows from max_len on are not attended), which sizes the
     split over workgroups and the workspace.  Returns out like q, zeros where no row is attended, and with return_softmax_lse the
     log-sum-exp [B, heads * gs] (-inf there).  `scratch`: the caller's own Scratch, where calls may overlap others."""
+    out = step_calls().paged_attention(q, k_pages, v_pages, block_table, cache_seqlens, starts, scores, scale, return_softmax_lse,
+                                       max_len, _held(q, "paged", scratch))
+    if out is not None:
+        return check(out, "paged_attention") if out.__class__ is int else out
     if not isinstance(q, torch.Tensor) or q.dim() != 4 or q.shape[1] != 1 or q.shape[0] < 1:
         raise ValueError("paged_attention: expected q [B, 1, heads, dim]")
     B, _, hq, dim = q.shape
@@ -939,6 +948,10 @@ def paged_append(key, value, k_pages, v_pages, block_table, cache_seqlens, new_s
     in each head, the first `sinks` and the last `recent` tokens of the sequence (the new one is the last) excepted; equal scores:
     the lowest row.  The row's score becomes 0, its position the token's.  A full sequence without scores is left as it is.
     new_seqlens [B] int32, another tensor than cache_seqlens: the rows in use afterwards."""
+    status = step_calls().paged_append(key, value, k_pages, v_pages, block_table, cache_seqlens, new_seqlens, scores, positions,
+                                       token_positions, budget, sinks, recent)
+    if status is not None:
+        return check(status, "paged_append") if status else None
     if not isinstance(key, torch.Tensor) or key.dim() != 4 or key.shape[1] != 1 or key.shape[0] < 1:
         raise ValueError("paged_append: expected key [B, 1, heads, dim]")
     B = key.shape[0]
@@ -975,6 +988,10 @@ def paged_fill(key, value, k_pages, v_pages, block_table, new_seqlens=None, seql
     `sinks`, the last `recent` and of the others those with the highest weights [B, heads, T] fp32 (attention_weights), at equal
     weights the first ones, in their order.  new_seqlens [B] int32: the rows written.  scores, positions [B, heads, rows]: take the
     kept weights and the tokens' places."""
+    status = step_calls().paged_fill(key, value, k_pages, v_pages, block_table, new_seqlens, seqlens, weights, scores, positions,
+                                     budget, sinks, recent, _held(key, "paged_fill", scratch))
+    if status is not None:
+        return check(status, "paged_fill") if status else None
     if not isinstance(key, torch.Tensor) or key.dim() != 4 or key.shape[0] < 1 or key.shape[1] < 1:
         raise ValueError("paged_fill: expected key [B, T, heads, dim]")
     B, T = key.shape[:2]
@@ -1011,6 +1028,9 @@ def attention_weights(q, key, seqlens=None, scale=None, scratch=None):
     heads of a key-value head: fp32 [B, heads, T], 0 past a prompt's end.  q [B, W, heads * gs, dim], the queries of the last W
     tokens (of all: W = T); key [B, T, heads, dim]; seqlens [B] int32: the prompts' lengths (default T), query i being that of token
     seqlens[b] - W + i (one before token 0 weighs nothing)."""
+    out = step_calls().attention_weights(q, key, seqlens, scale, _held(key, "weights", scratch))
+    if out is not None:
+        return check(out, "attention_weights") if out.__class__ is int else out
     if not isinstance(q, torch.Tensor) or not isinstance(key, torch.Tensor) or q.dim() != 4 or key.dim() != 4 or not key.is_cuda:
         raise ValueError("attention_weights: expected device tensors q [B, W, heads * gs, dim] and key [B, T, heads, dim]")
     if key.dtype not in _DT:

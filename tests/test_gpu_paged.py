@@ -243,6 +243,10 @@ def test_append_without_scores_and_with_odd_ones(dev):
     (BF, 2, 1030, 1, 128, 16, 100, [1030, 99], 1, 0, "zero"),
     (BF, 1, 4097, 2, 64, 256, 1, None, 0, 0, "odd"),
     (BF, 1, 70000, 2, 64, 256, 9000, None, 4, 64, "any"),
+    (HF, 4, 9001, 2, 64, 64, 700, [9001, 4096, 4097, 100], 4, 64, "any"),
+    (BF, 2, 8200, 1, 64, 32, 8100, None, 0, 4100, "zero"),
+    (BF, 1, 12289, 2, 64, 32, 5000, [12288], 0, 0, "few"),
+    (HF, 1, 16384, 1, 64, 128, 4097, None, 17, 0, "odd"),
 ])
 def test_fill(dev, dt, B, T, heads, dim, page, budget, lens, sinks, recent, weights):
     gen = torch.Generator().manual_seed(T + page)
@@ -281,6 +285,28 @@ def test_fill(dev, dt, B, T, heads, dim, page, budget, lens, sinks, recent, weig
         assert torch.equal(got.cpu(), want)
     if scores is not None:
         assert torch.equal(d[3].cpu().nan_to_num(-77), scores.nan_to_num(-77))
+
+
+def test_fill_of_a_prompt_of_many_chunks(dev):
+    """More than 1024 chunks of 4096 rows, equal weights among them."""
+    T, budget, sinks, recent = 4_300_001, 70_000, 4, 100
+    gen = torch.Generator(device=dev).manual_seed(11)
+    w = torch.rand(1, 1, T, generator=gen, device=dev)
+    w[..., ::3] = 0.99
+    key = torch.randn(1, T, 1, 64, generator=gen, device=dev).to(BF)
+    per = -(-budget // 256)
+    table = torch.randperm(per, generator=gen, device=dev).view(1, per).to(torch.int32)
+    k, v = torch.zeros(per, 1, 256, 64, dtype=BF, device=dev), torch.zeros(per, 1, 256, 64, dtype=BF, device=dev)
+    positions = torch.zeros(1, 1, budget, dtype=torch.int32, device=dev)
+    scores = torch.zeros(1, 1, budget, device=dev)
+    kernels.paged_fill(key, key, k, v, table, weights=w, scores=scores, positions=positions, budget=budget, sinks=sinks, recent=recent)
+    x = w[0, 0].clone()
+    x[:sinks] = x[T - recent:] = 2.0
+    want = torch.sort(x, descending=True, stable=True).indices[:budget].sort().values
+    assert torch.equal(positions[0, 0].long(), want) and torch.equal(scores[0, 0], w[0, 0, want])
+    r = torch.arange(budget, device=dev)
+    at = table[0].long()[r // 256]
+    assert torch.equal(k[at, 0, r % 256], key[0, want, 0]) and torch.equal(v[at, 0, r % 256], key[0, want, 0])
 
 
 # ------------------------------------------------------------------------------------------------ weights of a prompt

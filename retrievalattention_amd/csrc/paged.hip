@@ -7,11 +7,13 @@
 #include "ri_common.h"
 
 #define PG_WAVES 8             // waves of an attending workgroup
-#define PG_ROWS_MIN 128        // rows of a workgroup at least: a chunk of 16 per wave
 #define PG_LOG2E 1.4426950408889634f
 #define PG_LN2 0.6931471805599453f
 
 typedef short pg_s4 __attribute__((ext_vector_type(4)));
+// four values, a row each, that need not be aligned to more than one
+typedef float pg_f4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef int pg_i4 __attribute__((ext_vector_type(4), aligned(4)));
 
 __device__ __forceinline__ float pg_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
@@ -32,10 +34,11 @@ struct PagedAttendParams {
   float* lse;             // [B, heads * gs] or null
   float* scores;          // [B, heads, ..] or null
   int64_t sb, sh;         // its strides
-  float* part_ml;         // [B * heads, S, GP, 2]: maximum (of scores in units of ln 2) and sum
-  float* part_acc;        // [B * heads, S, GP, D]
+  float* part_ml;         // [workgroups + B * heads, GP, 2]: maximum (of scores in units of ln 2) and sum of a part
+  float* part_acc;        // [workgroups + B * heads, GP, D]
   float* logits;          // [B * heads, gs, max_len], units of ln 2
-  int gs, S, rows, max_len;   // rows: of a workgroup, a multiple of 16
+  int B, gs, max_len;
+  int workgroups;         // that share the rows; 0: one to each group, which writes the output
   float scale2;           // scale / ln 2
 };
 
@@ -60,14 +63,81 @@ __device__ __forceinline__ f32x4_t pg_mfma16(pg_s4 a, pg_s4 b, f32x4_t c) {
 __device__ __forceinline__ float pg_row_max(float x) { return ri_xor_max<1>(ri_xor_max<2>(ri_xor_max<4>(ri_xor_max<8>(x)))); }
 __device__ __forceinline__ float pg_row_sum(float x) { return ri_xor_sum<1>(ri_xor_sum<2>(ri_xor_sum<4>(ri_xor_sum<8>(x)))); }
 
+// The rows of all groups, (sequence, key-value head) pairs in order, are one run of chunks of 16, of which workgroup i takes a
+// share of `each`, whatever the lengths: places [i each, (i + 1) each).  A group that has rows begins with PG_LEAD places without
+// any, about what its query, its merge and its part cost (a workgroup with a dozen short groups was what all others waited for).
+// What workgroup i has of group g is part i + g: along the run either i or g moves on, so no two are the same.
+#define PG_SHARE 32   // places of a share at least
+#define PG_LEAD 32
+// places of a group of sequence b
+__device__ __forceinline__ int pg_places(const PagedAttendParams& P, int b) {
+  int first, last;
+  pg_range(P, b, &first, &last);
+  return first < last ? ((last + 15) >> 4) - (first >> 4) + PG_LEAD : 0;
+}
+struct PagedRun {
+  int64_t each, total;   // places of a workgroup's share and of all groups
+  int64_t from;          // those of one head in front of sequence b's
+  int b;
+};
+// x, from which nothing that the compiler knows is to be kept in registers over what stands before
+__device__ __forceinline__ int pg_anew(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+__device__ __forceinline__ int64_t pg_uniform(int64_t x) {
+  return (int64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)x) | (int64_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32;
+}
+// Whole workgroup of THREADS: the run, and of the sequences the one for which is_it(b, from, places, each) holds.
+template <int THREADS, typename IsIt>
+__device__ __forceinline__ PagedRun pg_run(const PagedAttendParams& P, IsIt&& is_it) {
+  constexpr int NW = THREADS / 64;
+  __shared__ uint32_t sh_wave[NW];
+  __shared__ int64_t sh_from;
+  __shared__ int sh_b;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const bool one = P.B <= THREADS;
+  int64_t sum = 0, each = 0;
+  for (int pass = one ? 1 : 0; pass < 2; ++pass) {   // the sum first; of few sequences everything at once
+    int64_t in_front = 0;
+    for (int b0 = 0; b0 < P.B; b0 += THREADS) {
+      const int b = b0 + (int)threadIdx.x, n = b < P.B ? pg_places(P, b) : 0;
+      const uint32_t incl = ri_wave_incl_scan((uint32_t)n);
+      __syncthreads();
+      if (lane == 63) sh_wave[wave] = incl;
+      __syncthreads();
+      uint32_t before = incl - n, all = 0;
+#pragma unroll
+      for (int i = 0; i < NW; ++i) {
+        const uint32_t x = sh_wave[i];
+        before += i < wave ? x : 0u;
+        all += x;
+      }
+      if (one) sum = all;
+      if (pass) {
+        const int64_t share = (sum * P.c.heads + P.workgroups - 1) / P.workgroups;
+        each = share < PG_SHARE ? PG_SHARE : share;
+        if (b < P.B && is_it(b, in_front + before, n, each)) {
+          sh_from = in_front + before;
+          sh_b = b;
+        }
+      }
+      in_front += all;
+    }
+    sum = in_front;
+  }
+  __syncthreads();
+  return {pg_uniform(each), pg_uniform(sum * P.c.heads), pg_uniform(sh_from), __builtin_amdgcn_readfirstlane(sh_b)};
+}
+
 // s = scale q.k, p = exp(s - m), out = sum p v / sum p over the rows of one (sequence, key-value head), one pass with the running
-// maximum m.  Grid (B * heads, S): a workgroup has the `rows` rows from blockIdx.y * rows on, each of its waves a run of them in
-// chunks of 16.  GP: query heads padded to 4, 8 or 16.  The products are MFMA 16x16x32 with the heads as rows of A (row m: head
-// m % GP) and 16 cache rows as columns of B: lane (n, h) = (lane % 16, lane / 16) gets the scores of cache row n for the heads
-// 4 h + i of A's rows, of which it keeps GP / 4, so that every (row, head) is some lane's once.
+// maximum m.  Each of a workgroup's waves takes a run of its chunks of 16 rows.  GP: query heads padded to 4, 8 or 16.  The products
+// are MFMA 16x16x32 with the heads as rows of A (row m: head m % GP) and 16 cache rows as columns of B: lane (n, h) = (lane % 16,
+// lane / 16) gets the scores of cache row n for the heads 4 h + i of A's rows, of which it keeps GP / 4, so that every (row, head) is
+// some lane's once.
 // UNI: a chunk lies in one page (pages of 16 rows and more), whose address is the same for the whole wave.
 template <int D, int GP, bool HALF, bool UNI>
-__global__ __launch_bounds__(64 * PG_WAVES, 4) void paged_attend_kernel(PagedAttendParams P) {
+__global__ __launch_bounds__(64 * PG_WAVES, UNI && GP < 16 ? 4 : 2) void paged_attend_kernel(PagedAttendParams P) {
   constexpr int NH = GP / 4, DT = D / 16, KK = D / 32, VS = D + 16;
   constexpr int LPR = D / 8, RPI = 64 / LPR, NV = 16 / RPI;   // lanes to a value row, value rows to a load, loads to a chunk
   constexpr int TILE = (16 * VS * 2 > GP * D * 4) ? 16 * VS * 2 : GP * D * 4;
@@ -76,22 +146,48 @@ __global__ __launch_bounds__(64 * PG_WAVES, 4) void paged_attend_kernel(PagedAtt
   __shared__ __attribute__((aligned(16))) float sh_al[PG_WAVES][16];
   __shared__ float sh_m[PG_WAVES][GP], sh_l[PG_WAVES][GP];
 
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int n = lane & 15, h = lane >> 4;
-  const int g = blockIdx.x, split = blockIdx.y;
-  const int b = g / P.c.heads, head = g - b * P.c.heads;
-  int first, last;
-  pg_range(P, b, &first, &last);
-  const int w0 = max(split * P.rows, first & ~15), w1 = min((split + 1) * P.rows, last);
-  if (P.S > 1 && w0 >= w1) return;   // (nothing of this workgroup is read)
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int b = blockIdx.x / P.c.heads, head = blockIdx.x - b * P.c.heads, skip = 0;   // skip: places of the group that are others'
+  int64_t at = 0, end = 0;        // this workgroup's places of the run that are still to be done
+  if (P.workgroups) {
+    const int64_t i = blockIdx.x, heads = P.c.heads;
+    const PagedRun run = pg_run<64 * PG_WAVES>(P, [&](int, int64_t from, int places, int64_t each) {
+      return from * heads <= i * each && i * each < (from + places) * heads;
+    });
+    at = i * run.each;
+    if (at >= run.total) return;
+    end = min(at + run.each, run.total);
+    b = run.b;
+    const int mine = (int)(at - run.from * heads), per_head = pg_places(P, b);
+    head = mine / per_head;
+    skip = mine - head * per_head;
+  }
 
   uint16_t* const vt = (uint16_t*)sh_tile[wave];
   uint16_t* const pb = sh_p[wave];
   float* const al_sh = sh_al[wave];
-  reinterpret_cast<uint2*>(pb)[lane] = make_uint2(0u, 0u);
-  if (lane < 16) al_sh[lane] = 1.f;
+  reinterpret_cast<uint2*>(pb)[threadIdx.x & 63] = make_uint2(0u, 0u);
+  if ((threadIdx.x & 63) < 16) al_sh[threadIdx.x & 63] = 1.f;
+  const int shift = P.c.shift, mask = P.c.mask;
+  const int upc = UNI ? 1 : 16 >> shift;      // units, of which a lane holds the page, to a chunk
+  const int ush = UNI ? 4 : shift;            // rows of a unit as a power of two
+  const int cpb = 64 / upc;                   // chunks to a batch of 64 units
 
-  const int hq = n % GP;
+  for (;;) {   // the groups that this workgroup has rows of
+  const int lane = pg_anew(threadIdx.x & 63), n = lane & 15, h = lane >> 4;
+  const int hq = n % GP, rsel = GP == 4 ? h : (GP == 8 ? (h >> 1) * 2 : 0);   // rsel: first accumulator register that this lane keeps
+  const auto head_of = [&](int i) { return (4 * h + rsel + i) % GP; };
+  const int g = b * P.c.heads + head;
+  int first, last;
+  pg_range(P, b, &first, &last);
+  int w0 = first & ~15, w1 = last;
+  if (P.workgroups) {
+    const int places = pg_places(P, b), mine = (int)min((int64_t)(places - skip), end - at);
+    w1 = min(w0 + (max(skip + mine - PG_LEAD, 0) << 4), last);
+    w0 += max(skip - PG_LEAD, 0) << 4;
+    at += mine;
+  }
+  if (w0 < w1 || !P.workgroups) {
   uint4 q[KK];
 #pragma unroll
   for (int kk = 0; kk < KK; ++kk)
@@ -103,8 +199,6 @@ __global__ __launch_bounds__(64 * PG_WAVES, 4) void paged_attend_kernel(PagedAtt
   for (int i = 0; i < NH; ++i) { m[i] = -INFINITY; l[i] = 0.f; }
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) acc[dt] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
-  const int rsel = GP == 4 ? h : (GP == 8 ? (h >> 1) * 2 : 0);   // first accumulator register that this lane keeps
-  const auto head_of = [&](int i) { return (4 * h + rsel + i) % GP; };
 
   // this wave's chunks [c0, c1) of 16 rows
   const int chunks = (w1 - w0 + 15) >> 4, per = (max(chunks, 0) + PG_WAVES - 1) / PG_WAVES;
@@ -112,99 +206,117 @@ __global__ __launch_bounds__(64 * PG_WAVES, 4) void paged_attend_kernel(PagedAtt
   const int32_t* const table = P.c.table + b * P.c.ts;
   const uint16_t* const kb = P.c.k + head * P.c.kh;
   const uint16_t* const vb = P.c.v + head * P.c.vh;
-  const int shift = P.c.shift, mask = P.c.mask;
-  const int upc = UNI ? 1 : 16 >> shift;      // units, of which a lane holds the page, to a chunk
-  const int ush = UNI ? 4 : shift;            // rows of a unit as a power of two
-  const int cpb = 64 / upc;                   // chunks to a batch of 64 units
-
-  for (int cb = c0; cb < c1; cb += cpb) {
-    // lane's unit of this batch: its page, -1 where there is none
-    int pid;
-    {
-      const int row = ((cb * upc) + lane) << ush;
-      const int at = row >> shift;
-      pid = row < w1 ? table[min(at, P.c.table_pages - 1)] : -1;
-      if ((unsigned)pid >= (unsigned)P.c.pages) pid = -1;
+  // the page of this lane's unit of the batch that begins with chunk c; -1 where there is none
+  const auto units = [&](int c) {
+    const int row = (c * upc + lane) << ush;
+    const int page = table[min(row >> shift, P.c.table_pages - 1)];
+    return row < w1 && (unsigned)page < (unsigned)P.c.pages ? page : -1;
+  };
+  // A chunk's keys and values are requested as soon as the registers of the one before are free, whether their rows are attended
+  // or not (rows of page 0 stand in for those of a page that is not there): no load is under a condition.
+  int cb = c0, pid = units(c0), pid_next = units(c0 + cpb);
+  int pk = -1, pv[NV];
+  uint4 k[KK], v[NV];
+  const uint32_t koff = (uint32_t)n * (uint32_t)P.c.kr + h * 8, voff = (uint32_t)(lane / LPR) * (uint32_t)P.c.vr + (lane % LPR) * 8;
+  const auto pages = [&](int c) {
+    if (c == cb + cpb) {
+      cb = c;
+      pid = pid_next;
+      pid_next = units(c + cpb);
     }
-    const int ce = min(c1, cb + cpb);
-    for (int c = cb; c < ce; ++c) {
-      const int r0 = c << 4;
-      uint4 k[KK], v[NV];
-      int pk, pv[NV];
-      if (UNI) {
-        pk = __builtin_amdgcn_readlane(pid, c - cb);
+    if (UNI) {
+      pk = __builtin_amdgcn_readlane(pid, c - cb);
+    } else {
+      pk = __shfl(pid, (c - cb) * upc + (n >> shift));
 #pragma unroll
-        for (int i = 0; i < NV; ++i) pv[i] = pk;
-      } else {
-        pk = __shfl(pid, (c - cb) * upc + (n >> shift));
+      for (int i = 0; i < NV; ++i) pv[i] = __shfl(pid, (c - cb) * upc + ((lane / LPR + RPI * i) >> shift));
+    }
+  };
+  const auto load_keys = [&](int c) {
+    const uint16_t* from = UNI ? kb + max(pk, 0) * P.c.kp + ((c << 4) & mask) * P.c.kr + koff
+                               : kb + max(pk, 0) * P.c.kp + (n & mask) * P.c.kr + h * 8;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) pv[i] = __shfl(pid, (c - cb) * upc + ((lane / LPR + RPI * i) >> shift));
-      }
-      const int rk = r0 + n;
-      const bool valid = pk >= 0 && rk >= first && rk < last;
-      const uint16_t* kp = kb + max(pk, 0) * P.c.kp + (rk & mask) * P.c.kr + h * 8;
+    for (int kk = 0; kk < KK; ++kk) k[kk] = ri_ld16(from + kk * 32);
+  };
+  const auto load_values = [&](int c) {
+    const uint16_t* from = vb + max(pk, 0) * P.c.vp + ((c << 4) & mask) * P.c.vr + voff;
 #pragma unroll
-      for (int kk = 0; kk < KK; ++kk) k[kk] = valid ? ri_ld16(kp + kk * 32) : ri_zero16();
+    for (int i = 0; i < NV; ++i)
+      v[i] = UNI ? ri_ld16(from + RPI * i * P.c.vr)
+                 : ri_ld16(vb + max(pv[i], 0) * P.c.vp + ((lane / LPR + RPI * i) & mask) * P.c.vr + (lane % LPR) * 8);
+  };
+  if (c0 < c1) {
+    pages(c0);
+    load_keys(c0);
+    load_values(c0);
+  }
+  for (int c = c0; c < c1; ++c) {
+    const int r0 = c << 4, rk = r0 + n;
+    const bool valid = pk >= 0 && rk >= first && rk < last;
+    f32x4_t s4 = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) s4 = pg_mfma32<HALF>(q[kk], k[kk], s4);
+    if (__builtin_amdgcn_ballot_w64(valid) != ~0ull) {   // values that are not attended bring no NaN into the products
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int rv = r0 + lane / LPR + RPI * i;
-        const bool ok = pv[i] >= 0 && rv >= first && rv < last;   // (rows that are not attended bring no NaN into the products)
-        v[i] = ok ? ri_ld16(vb + max(pv[i], 0) * P.c.vp + (rv & mask) * P.c.vr + (lane % LPR) * 8) : ri_zero16();
+        if ((UNI ? pk : pv[i]) < 0 || rv < first || rv >= last) v[i] = ri_zero16();
       }
-      f32x4_t s4 = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+    }
 #pragma unroll
-      for (int kk = 0; kk < KK; ++kk) s4 = pg_mfma32<HALF>(q[kk], k[kk], s4);
+    for (int i = 0; i < NV; ++i) *reinterpret_cast<uint4*>(vt + (lane / LPR + RPI * i) * VS + (lane % LPR) * 8) = v[i];
+    if (c + 1 < c1) {
+      pages(c + 1);
+      load_keys(c + 1);
+      load_values(c + 1);
+    }
+    float al[NH];
+    bool rescale = false;
 #pragma unroll
-      for (int i = 0; i < NV; ++i)
-        *reinterpret_cast<uint4*>(vt + (lane / LPR + RPI * i) * VS + (lane % LPR) * 8) = v[i];
-      float al[NH];
-      bool rescale = false;
+    for (int i = 0; i < NH; ++i) {
+      const int r = GP == 16 ? i : rsel + i;
+      const float x = r == 0 ? s4[0] : r == 1 ? s4[1] : r == 2 ? s4[2] : s4[3];
+      const float s = valid ? x * P.scale2 : -INFINITY;
+      if (P.logits && rk < w1 && head_of(i) < P.gs) P.logits[((size_t)g * P.gs + head_of(i)) * P.max_len + rk] = s;
+      const float mn = fmaxf(m[i], pg_row_max(s));
+      const bool none = mn == -INFINITY;   // relative to -inf they would weigh NaN
+      al[i] = none ? 1.f : pg_exp2(m[i] - mn);
+      const float p = pg_exp2(s - (none ? 0.f : mn));
+      rescale |= al[i] != 1.f;
+      l[i] = l[i] * al[i] + p;
+      m[i] = mn;
+      pb[head_of(i) * 16 + n] = ri_f32_to_e16<HALF>(p);
+    }
+    const bool any = __builtin_amdgcn_ballot_w64(rescale) != 0;
+    if (any && n == 0) {
 #pragma unroll
-      for (int i = 0; i < NH; ++i) {
-        const int r = GP == 16 ? i : rsel + i;
-        const float x = r == 0 ? s4[0] : r == 1 ? s4[1] : r == 2 ? s4[2] : s4[3];
-        const float s = valid ? x * P.scale2 : -INFINITY;
-        if (P.logits && rk < w1 && head_of(i) < P.gs)
-          P.logits[((size_t)g * P.gs + head_of(i)) * P.max_len + rk] = s;
-        const float mn = fmaxf(m[i], pg_row_max(s));
-        const bool none = mn == -INFINITY;   // relative to -inf they would weigh NaN
-        al[i] = none ? 1.f : pg_exp2(m[i] - mn);
-        const float p = pg_exp2(s - (none ? 0.f : mn));
-        rescale |= al[i] != 1.f;
-        l[i] = l[i] * al[i] + p;
-        m[i] = mn;
-        pb[head_of(i) * 16 + n] = ri_f32_to_e16<HALF>(p);
-      }
-      const bool any = __builtin_amdgcn_ballot_w64(rescale) != 0;
-      if (any && n == 0) {
-#pragma unroll
-        for (int i = 0; i < NH; ++i) al_sh[head_of(i)] = al[i];
-      }
-      ri_wave_sync();
-      if (any) {
-        const float4 a4 = *reinterpret_cast<const float4*>(al_sh + 4 * h);
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-          acc[dt][0] *= a4.x; acc[dt][1] *= a4.y; acc[dt][2] *= a4.z; acc[dt][3] *= a4.w;
-        }
-      }
-      // lane (n, h): P of head n and rows 4 h .., V of those rows and dim 16 dt + n by transpose reads
-      const pg_s4 pa = *reinterpret_cast<const pg_s4*>(pb + n * 16 + 4 * h);
-      const uint16_t* vsrc = vt + (4 * h + (n >> 2)) * VS + 4 * (n & 3);
+      for (int i = 0; i < NH; ++i) al_sh[head_of(i)] = al[i];
+    }
+    ri_wave_sync();
+    if (any) {
+      const float4 a4 = *reinterpret_cast<const float4*>(al_sh + 4 * h);
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
-        const pg_s4 vv = __builtin_amdgcn_ds_read_tr16_b64_v4i16((pg_s4 __attribute__((address_space(3)))*)(vsrc + 16 * dt));
-        acc[dt] = pg_mfma16<HALF>(pa, vv, acc[dt]);
+        acc[dt][0] *= a4.x; acc[dt][1] *= a4.y; acc[dt][2] *= a4.z; acc[dt][3] *= a4.w;
       }
-      ri_wave_sync();
     }
+    // lane (n, h): P of head n and rows 4 h .., V of those rows and dim 16 dt + n by transpose reads
+    const pg_s4 pa = *reinterpret_cast<const pg_s4*>(pb + n * 16 + 4 * h);
+    const uint16_t* vsrc = vt + (4 * h + (n >> 2)) * VS + 4 * (n & 3);
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      const pg_s4 vv = __builtin_amdgcn_ds_read_tr16_b64_v4i16((pg_s4 __attribute__((address_space(3)))*)(vsrc + 16 * dt));
+      acc[dt] = pg_mfma16<HALF>(pa, vv, acc[dt]);
+    }
+    ri_wave_sync();
   }
 
   // the waves merge in LDS
+  const int tid = pg_anew(threadIdx.x), n2 = tid & 15, h2 = (tid & 63) >> 4;
 #pragma unroll
   for (int i = 0; i < NH; ++i) {
     const float s = pg_row_sum(l[i]);
-    if (n == 0) {
+    if (n2 == 0) {
       sh_m[wave][head_of(i)] = m[i];
       sh_l[wave][head_of(i)] = s;
     }
@@ -212,14 +324,14 @@ __global__ __launch_bounds__(64 * PG_WAVES, 4) void paged_attend_kernel(PagedAtt
   float* const mine = (float*)sh_tile[wave];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int hd = 4 * h + i;
+    const int hd = 4 * h2 + i;
     if (hd < GP) {
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) mine[hd * D + 16 * dt + n] = acc[dt][i];
+      for (int dt = 0; dt < DT; ++dt) mine[hd * D + 16 * dt + n2] = acc[dt][i];
     }
   }
   __syncthreads();
-  for (int at = threadIdx.x; at < P.gs * D; at += 64 * PG_WAVES) {
+  for (int at = tid; at < P.gs * D; at += 64 * PG_WAVES) {
     const int j = at / D, d = at % D;
     float M = -INFINITY, L = 0.f, A = 0.f;
 #pragma unroll
@@ -230,82 +342,141 @@ __global__ __launch_bounds__(64 * PG_WAVES, 4) void paged_attend_kernel(PagedAtt
       L += sh_l[w][j] * f;
       A += ((const float*)sh_tile[w])[j * D + d] * f;
     }
-    const size_t o = (size_t)g * P.gs + j, part = ((size_t)g * P.S + split) * GP + j;
-    if (P.S == 1) {
-      P.out[o * D + d] = ri_f32_to_e16<HALF>(L > 0.f ? A / L : 0.f);
-      if (d == 0 && P.lse) P.lse[o] = L > 0.f ? (M + __log2f(L)) * PG_LN2 : -INFINITY;
-    } else {
+    const size_t o = (size_t)g * P.gs + j, part = (g + (P.workgroups ? (size_t)blockIdx.x : 0)) * GP + j;
+    if (P.workgroups) {
       P.part_acc[part * D + d] = A;
+    } else {
+      P.out[o * D + d] = ri_f32_to_e16<HALF>(L == 0.f ? 0.f : A / L);
+      if (d == 0 && P.lse) P.lse[o] = L == 0.f ? -INFINITY : (M + __log2f(L)) * PG_LN2;
     }
-    if (d == 0 && (P.S > 1 || P.logits)) {
+    if (d == 0 && (P.workgroups || P.logits)) {
       P.part_ml[2 * part] = M;
       P.part_ml[2 * part + 1] = L;
     }
   }
+  }
+  if (at >= end) return;
+  do {
+    if (++head == P.c.heads) { head = 0; ++b; }
+  } while (pg_places(P, b) == 0);   // (there are places left, so there is such a group)
+  skip = 0;
+  __syncthreads();
+  }
 }
 
 #define PG_JOIN_THREADS 256
-#define PG_JOIN_ROWS 1024      // scores of a workgroup of the join
+#define PG_JOIN_ROWS (4 * PG_JOIN_THREADS)   // scores of a workgroup of the join, four to a thread
+#define PG_WORKGROUPS 1024                   // that share the rows at most: parts of a group
 
-// Grid (B * heads, (S > 1 ? gs : 0) + ceil(max_len / PG_JOIN_ROWS) with scores): the first gs workgroups of a group join the
+// Grid (B * heads, (workgroups ? gs : 0) + ceil(max_len / PG_JOIN_ROWS) with scores): the first gs workgroups of a group join the
 // parts of a head each; the others add the weights of PG_JOIN_ROWS rows, exp(s - lse) summed over the heads, to the scores.
 template <int D, int GP, bool HALF>
 __global__ __launch_bounds__(PG_JOIN_THREADS) void paged_join_kernel(PagedAttendParams P) {
-  constexpr int PARTS = PG_JOIN_THREADS / D;
-  __shared__ float sh_M[16], sh_L[16], sh_a[PARTS][D];
+  constexpr int NW = PG_JOIN_THREADS / 64, U = 8, DL = D / 64;   // DL: dims of a lane; U: parts requested at a time
+  __shared__ float sh_M[16], sh_L[16], sh_f[PG_WORKGROUPS], sh_a[NW][D];
   const int g = blockIdx.x, b = g / P.c.heads, head = g - b * P.c.heads;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int first, last;
   pg_range(P, b, &first, &last);
-  const int s0 = P.S > 1 ? first / P.rows : 0, s1 = P.S > 1 ? (last + P.rows - 1) / P.rows : 1;   // splits that have rows
-  const int outs = P.S > 1 ? P.gs : 0;
+  const int outs = P.workgroups ? P.gs : 0;
   const bool joins = (int)blockIdx.y < outs;
-  const float* const ml = P.part_ml + (size_t)g * P.S * GP * 2;
-  for (int j = joins ? blockIdx.y + wave : wave; j < (joins ? (int)blockIdx.y + 1 : P.gs); j += PG_JOIN_THREADS / 64) {
+  const int r0 = ((int)blockIdx.y - outs) * PG_JOIN_ROWS;
+  if (!joins && (r0 >= last || r0 + PG_JOIN_ROWS <= first)) return;
+  int64_t s0 = 0, s1 = first < last;   // the workgroups that have rows of the group
+  if (P.workgroups && first < last) {
+    const PagedRun run = pg_run<PG_JOIN_THREADS>(P, [&](int seq, int64_t, int, int64_t) { return seq == b; });
+    const int places = pg_places(P, b);
+    const int64_t start = run.from * P.c.heads + (int64_t)head * places;
+    s0 = (start + PG_LEAD) / run.each;
+    s1 = (start + places - 1) / run.each + 1;
+  }
+  const int parts = (int)(s1 - s0);
+  const size_t part0 = (size_t)(g + s0);
+  const float2* const ml = reinterpret_cast<const float2*>(P.part_ml) + part0 * GP;
+  // maximum and sum of a head's parts, by a wave
+  const auto join = [&](int j) {
     float M = -INFINITY, L = 0.f;
-    if (first < last) {
-      for (int s = s0 + lane; s < s1; s += 64) M = fmaxf(M, ml[((size_t)s * GP + j) * 2]);
-      M = ri_wave_max(M);
-      if (M != -INFINITY)
-        for (int s = s0 + lane; s < s1; s += 64) L += ml[((size_t)s * GP + j) * 2 + 1] * pg_exp2(ml[((size_t)s * GP + j) * 2] - M);
-      L = ri_wave_sum(L);
-    }
+    for (int s = lane; s < parts; s += 64) M = fmaxf(M, ml[(size_t)s * GP + j].x);
+    M = ri_wave_max(M);
+    if (M != -INFINITY)
+      for (int s = lane; s < parts; s += 64) {
+        const float2 x = ml[(size_t)s * GP + j];
+        const float f = pg_exp2(x.x - M);
+        if (joins) sh_f[s] = f;
+        L += x.y * f;
+      }
+    L = ri_wave_sum(L);
     if (lane == 0) {
       sh_M[j] = M;
       sh_L[j] = L;
     }
-  }
-  __syncthreads();
+  };
   if (joins) {
-    const int j = blockIdx.y, d = threadIdx.x % D, p = threadIdx.x / D;
-    const float M = sh_M[j], L = sh_L[j];
-    const float* const acc = P.part_acc + (size_t)g * P.S * GP * D;
-    float A = 0.f;
-    if (L > 0.f)
-      for (int s = s0 + p; s < s1; s += PARTS) {
-        const float ms = ml[((size_t)s * GP + j) * 2];
-        A += acc[((size_t)s * GP + j) * D + d] * pg_exp2(ms - M);
-      }
-    sh_a[p][d] = A;
+    const int j = blockIdx.y;
+    if (wave == 0) join(j);
     __syncthreads();
-    if (p == 0) {
-      for (int i = 1; i < PARTS; ++i) A += sh_a[i][d];
-      const size_t o = (size_t)g * P.gs + j;
-      P.out[o * D + d] = ri_f32_to_e16<HALF>(L > 0.f ? A / L : 0.f);
-      if (d == 0 && P.lse) P.lse[o] = L > 0.f ? (M + __log2f(L)) * PG_LN2 : -INFINITY;
+    const float M = sh_M[j], L = sh_L[j];
+    float A[DL] = {};
+    if (M != -INFINITY) {
+      const float* const acc = P.part_acc + (part0 * GP + j) * D + DL * lane;
+      for (int s = wave; s < parts; s += U * NW) {
+        float x[U][DL];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int d = 0; d < DL; ++d) x[u][d] = acc[(size_t)min(s + u * NW, parts - 1) * GP * D + d];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (s + u * NW < parts) {
+#pragma unroll
+            for (int d = 0; d < DL; ++d) A[d] += x[u][d] * sh_f[s + u * NW];
+          }
+      }
     }
+#pragma unroll
+    for (int d = 0; d < DL; ++d) sh_a[wave][DL * lane + d] = A[d];
+    __syncthreads();
+    const size_t o = (size_t)g * P.gs + j;
+    for (int d = threadIdx.x; d < D; d += PG_JOIN_THREADS) {
+      float x = 0.f;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) x += sh_a[w][d];
+      P.out[o * D + d] = ri_f32_to_e16<HALF>(L == 0.f ? 0.f : x / L);
+    }
+    if (threadIdx.x == 0 && P.lse) P.lse[o] = L == 0.f ? -INFINITY : (M + __log2f(L)) * PG_LN2;
     return;
   }
-  const int r0 = ((int)blockIdx.y - outs) * PG_JOIN_ROWS;
-  float* const scores = P.scores + b * P.sb + head * P.sh;
-  for (int r = r0 + threadIdx.x; r < min(r0 + PG_JOIN_ROWS, last); r += PG_JOIN_THREADS) {
-    if (r < first) continue;
-    float w = 0.f;
-    for (int j = 0; j < P.gs; ++j) {
-      const float x = P.logits[((size_t)g * P.gs + j) * P.max_len + r];
-      w += sh_L[j] > 0.f ? pg_exp2(x - sh_M[j]) / sh_L[j] : 0.f;
+  const int r = r0 + 4 * threadIdx.x;
+  float* const scores = P.scores + b * P.sb + head * P.sh + r;
+  const float* const logits = P.logits + (size_t)g * P.gs * P.max_len + r;
+  const bool whole = r >= first && r + 4 <= last;
+  pg_f4 x[GP], was;
+  if (whole) {
+    was = *reinterpret_cast<const pg_f4*>(scores);
+#pragma unroll
+    for (int j = 0; j < GP; ++j) x[j] = *reinterpret_cast<const pg_f4*>(logits + (size_t)min(j, P.gs - 1) * P.max_len);
+  }
+  for (int j = wave; j < P.gs; j += NW) join(j);
+  __syncthreads();
+  if (whole) {
+#pragma unroll
+    for (int j = 0; j < GP; ++j) {
+      const float M = sh_M[min(j, P.gs - 1)], L = sh_L[min(j, P.gs - 1)], inv = j < P.gs && L != 0.f ? 1.f / L : 0.f;
+      if (inv != 0.f)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) was[i] += pg_exp2(x[j][i] - M) * inv;
     }
-    scores[r] += w;
+    *reinterpret_cast<pg_f4*>(scores) = was;
+  } else {
+    for (int i = 0; i < 4; ++i) {
+      if (r + i < first || r + i >= last) continue;
+      float w = scores[i];
+      for (int j = 0; j < P.gs; ++j) {
+        const float L = sh_L[j], inv = L != 0.f ? 1.f / L : 0.f;
+        if (inv != 0.f) w += pg_exp2(logits[(size_t)j * P.max_len + i] - sh_M[j]) * inv;
+      }
+      scores[i] = w;
+    }
   }
 }
 
@@ -330,10 +501,6 @@ struct PagedAppendParams {
   const int32_t* token;   // [B] position of the token that comes
   int budget, sinks, recent, dim;
 };
-
-// four values to a row that need not be aligned to more than one
-typedef float pg_f4 __attribute__((ext_vector_type(4), aligned(4)));
-typedef int pg_i4 __attribute__((ext_vector_type(4), aligned(4)));
 
 // Grid (heads, B).  The search for the weakest row reads eight bytes to a row, four rows to a lane's load and U loads ahead.
 template <int THREADS, int U>
@@ -724,6 +891,7 @@ static int paged_view(const ri_paged_t* c, int B, PagedView* v) {
     return RI_ERR_ARG;
   if (!strides_ok(c->k_page_stride, c->k_head_stride, c->k_row_stride) || !strides_ok(c->v_page_stride, c->v_head_stride, c->v_row_stride))
     return RI_ERR_ARG;
+  if (c->k_row_stride > 1 << 24 || c->v_row_stride > 1 << 24) return RI_ERR_ARG;   // (sixteen rows are addressed by 32 bits)
   if (c->heads > 65535 || B > 65535) return RI_ERR_ARG;   // (dimensions of grids)
   *v = {(const uint16_t*)c->k_pages, (const uint16_t*)c->v_pages, c->block_table, c->k_page_stride, c->k_head_stride, c->k_row_stride,
         c->v_page_stride, c->v_head_stride, c->v_row_stride, c->table_stride, c->pages, c->heads, __builtin_ctz(c->page_rows),
@@ -733,24 +901,29 @@ static int paged_view(const ri_paged_t* c, int B, PagedView* v) {
 
 static int pg_pad(int gs) { return gs <= 4 ? 4 : gs <= 8 ? 8 : 16; }
 
-// Rows of a workgroup: enough workgroups for the compute units, at least a chunk to a wave.
-static int paged_rows(int64_t groups, int max_len) {
-  const int64_t want = (groups * max_len + 1023) / 1024;
-  const int64_t rows = (want + PG_ROWS_MIN - 1) / PG_ROWS_MIN * PG_ROWS_MIN;
-  return (int)(rows < 512 ? 512 : rows);
+// Workgroups that share the rows: two to a compute unit, as many as run at a time, and twice as many from 128 groups on, of which
+// shares then are small parts (16 sequences of 1 .. 61440 tokens, 4 heads: 35 .. 95 us with 512, 41 .. 98 with 1024; 32 sequences of
+// 4096, 8 heads: 118 and 112).  None up to 512 rows: one to each group then, which leaves nothing to join (8 groups of 331 rows 8.2
+// us, shared 10 + 4).
+static int paged_workgroups(int64_t groups, int max_len) {
+  if (max_len <= 512) return 0;
+  const int64_t shares = (groups * ((max_len + 15) / 16 + 1 + PG_LEAD) + PG_SHARE - 1) / PG_SHARE;
+  const int most = groups < 128 ? PG_WORKGROUPS / 2 : PG_WORKGROUPS;
+  return (int)(shares < most ? shares : most);
 }
 
 extern "C" size_t ri_paged_attention_workspace_bytes(int B, int heads, int gs, int dim, int max_len, int scored) {
-  if (B <= 0 || heads <= 0 || gs <= 0 || gs > 16 || max_len <= 0 || (dim != 64 && dim != 128)) return 0;
-  const size_t groups = (size_t)B * heads, S = ((size_t)max_len + paged_rows(groups, max_len) - 1) / paged_rows(groups, max_len);
-  return groups * S * pg_pad(gs) * (2 + dim) * sizeof(float) + (scored ? groups * gs * max_len * sizeof(float) : 0);
+  if (B <= 0 || heads <= 0 || gs <= 0 || gs > 16 || max_len <= 0 || max_len > PG_MAX_ROWS || (dim != 64 && dim != 128)) return 0;
+  const int64_t groups = (int64_t)B * heads;
+  const size_t parts = groups + paged_workgroups(groups, max_len);
+  return parts * pg_pad(gs) * (2 + dim) * sizeof(float) + (scored ? (size_t)groups * gs * max_len * sizeof(float) : 0);
 }
 
 template <int D, int GP, bool HALF>
 static void launch_paged(const PagedAttendParams& P, int groups, hipStream_t s) {
   auto* kernel = P.c.shift >= 4 ? paged_attend_kernel<D, GP, HALF, true> : paged_attend_kernel<D, GP, HALF, false>;
-  kernel<<<dim3(groups, P.S), 64 * PG_WAVES, 0, s>>>(P);
-  const int y = (P.S > 1 ? P.gs : 0) + (P.scores ? (P.max_len + PG_JOIN_ROWS - 1) / PG_JOIN_ROWS : 0);
+  kernel<<<P.workgroups ? P.workgroups : groups, 64 * PG_WAVES, 0, s>>>(P);
+  const int y = (P.workgroups ? P.gs : 0) + (P.scores ? (P.max_len + PG_JOIN_ROWS - 1) / PG_JOIN_ROWS : 0);
   if (y) paged_join_kernel<D, GP, HALF><<<dim3(groups, y), PG_JOIN_THREADS, 0, s>>>(P);
 }
 
@@ -770,7 +943,8 @@ extern "C" int ri_paged_attention(const ri_paged_t* cache, const void* q, const 
   if (const int rc = paged_view(cache, B, &P.c)) return rc;
   if (!q || !lens || !out || !workspace || ri_any_misaligned16(q, out, workspace)) return RI_ERR_ARG;
   const int64_t groups = (int64_t)B * cache->heads;
-  if (gs <= 0 || gs > 16 || max_len <= 0 || max_len > cache->table_pages * cache->page_rows || groups > INT32_MAX / 16) return RI_ERR_ARG;
+  if (gs <= 0 || gs > 16 || max_len <= 0 || max_len > cache->table_pages * cache->page_rows || groups > INT32_MAX / 16 || (int64_t)B * (max_len / 16 + 2 + PG_LEAD) > INT32_MAX)
+    return RI_ERR_ARG;   // (places of all sequences are counted in 32 bits)
   if (scores && (score_batch_stride < 0 || score_head_stride < max_len)) return RI_ERR_ARG;
   if (workspace_bytes < ri_paged_attention_workspace_bytes(B, cache->heads, gs, cache->dim, max_len, scores != nullptr))
     return RI_ERR_WORKSPACE;
@@ -784,10 +958,10 @@ extern "C" int ri_paged_attention(const ri_paged_t* cache, const void* q, const 
   P.sh = score_head_stride;
   P.gs = gs;
   P.max_len = max_len;
-  P.rows = paged_rows(groups, max_len);
-  P.S = (max_len + P.rows - 1) / P.rows;
+  P.B = B;
+  P.workgroups = paged_workgroups(groups, max_len);
   P.scale2 = scale * PG_LOG2E;
-  const size_t parts = (size_t)groups * P.S * pg_pad(gs);
+  const size_t parts = (size_t)(groups + P.workgroups) * pg_pad(gs);
   P.part_ml = (float*)workspace;
   P.part_acc = P.part_ml + 2 * parts;
   P.logits = scores ? P.part_acc + parts * cache->dim : nullptr;

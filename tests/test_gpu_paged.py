@@ -84,6 +84,11 @@ CASES = [
     (BF, 2, 1, 9, 64, 256, [1500, 700], [700, 0]),
     (BF, 1, 2, 4, 128, 16, [5003], None),
     (HF, 2, 1, 12, 128, 2, [1111, 0], [1, 0]),
+    # rows shared over workgroups: empty sequences first, between and last, parts of several groups in one share
+    (BF, 7, 3, 4, 128, 16, [0, 3001, 0, 0, 17, 600, 0], [0, 5, 0, 0, 17, 590, 0]),
+    (HF, 5, 2, 1, 64, 8, [1, 1025, 2049, 513, 0], None),
+    (BF, 1, 1, 2, 64, 32, [0], None),
+    (BF, 70, 1, 4, 64, 16, [(37 * i) % 640 for i in range(70)], [(37 * i) % 640 // 2 for i in range(70)]),
 ]
 
 
@@ -91,7 +96,7 @@ CASES = [
 @pytest.mark.parametrize("scored", [False, True])
 def test_attention(dev, dt, B, heads, gs, dim, page, lens, starts, scored):
     gen = torch.Generator().manual_seed(B * 1000 + dim + page + lens[0])
-    rows = max(lens) + 3
+    rows = max(lens) + 3 if B < 7 else max(max(lens), 600) + 3
     k, v, table = _pool(gen, dt, B, heads, dim, page, rows)
     lens, starts = torch.tensor(lens, dtype=torch.int32), None if starts is None else torch.tensor(starts, dtype=torch.int32)
     _spoil(k, v, table, lens, starts)
@@ -123,6 +128,22 @@ def test_attention_max_len_scale_and_strides(dev):
     out, lse = kernels.paged_attention(q.to(dev), k, v, table, lens.to(dev), scale=0.2, max_len=77, return_softmax_lse=True)
     _check_attention(q, k.cpu(), v.cpu(), table.cpu(), lens.clamp(max=77), None, out, lse, 0.2)
     assert bool((out[2] == 0).all()) and bool((lse[2] == -math.inf).all())
+
+
+@pytest.mark.parametrize("B,room", [(600, 1024), (1300, 640)])
+def test_attention_of_many_sequences(dev, B, room):
+    """More sequences than a workgroup looks at at a time; most of them empty or short."""
+    gen = torch.Generator().manual_seed(B)
+    lens = torch.where(torch.rand(B, generator=gen) < 0.5, 0, (torch.rand(B, generator=gen) ** 6 * room).int()).to(torch.int32)
+    lens[-1], lens[B // 2] = room, 513
+    per, page = room // 64, 64
+    k, v = _randn(gen, 40, 2, page, 64).to(BF), _randn(gen, 40, 2, page, 64).to(BF)
+    table = torch.randint(40, (B, per), generator=gen).to(torch.int32)   # pages that sequences share
+    q = _randn(gen, B, 1, 4, 64).to(BF)
+    before = torch.rand(B, 2, room, generator=gen)
+    scores = before.to(dev)
+    out, lse = kernels.paged_attention(*(t.to(dev) for t in (q, k, v, table, lens)), scores=scores, return_softmax_lse=True)
+    _check_attention(q, k, v, table, lens, None, out, lse, 0.125, before, scores)
 
 
 def test_attention_of_extreme_scores(dev):

@@ -4,21 +4,22 @@ inference, model_hub/llama.py:222-346 the per-layer operators), with randomly in
 (there are no checkpoints to load here).  Everything outside the attention is stock torch: RMSNorm,
 the fused QKV projection, rotary embedding, the output projection and the SwiGLU MLP.
 
-Two attention back-ends, as in the reference's attention_type switch:
+Attention back-ends, the first two as in the reference's attention_type switch:
   "RetroInfer"       the wave-index cache of this package (cache_hub.retroinfer_cache)
   "Full_Flash_Attn"  plain attention over a dense K/V cache (the baseline the reference compares with)
+  "Paged_Attn"       attention over a paged K/V cache, with a budget of rows where one is given (cache_hub.paged_cache)
 
 A whole decoded token (every layer) can be captured into one HIP graph and replayed token after
-token: the wave-index cache is then built with device_positions=True, and the rotary position comes
-from a device-side counter.
+token: the wave-index cache is then built with device_positions=True (a paged cache is ready for it: its prepare_token() goes
+before each replay), and the rotary position comes from a device-side counter.
 """
 import math
 from dataclasses import dataclass
 
 import torch
 
-from ..attn_hub import retroinfer_prefill_attn, retroinfer_decode_attn
-from ..cache_hub import retroinfer_cache
+from ..attn_hub import paged_decode_attn, retroinfer_prefill_attn, retroinfer_decode_attn
+from ..cache_hub import paged_cache, retroinfer_cache
 
 
 @dataclass
@@ -132,11 +133,16 @@ class LlamaModel:
     def init_kv_cache(self, attention_type, batch_size, input_length, max_new_length, attn_config=None,
                       device_positions=False):
         """attn_config: n_centroids, n_segment, nprobe, max_compute_cluster_num, cache_cluster_num
-        (reference: llama.py:154-211 reads them from config/<model>.json)."""
+        (reference: llama.py:154-211 reads them from config/<model>.json); for "Paged_Attn" the options of paged_cache:
+        page_size, budget, sinks, recent, window, pages."""
         self.attention_type = attention_type
         if attention_type == "Full_Flash_Attn":
             self.kv_cache = DenseCache(self.num_layers, batch_size, input_length + max_new_length,
                                        self.num_key_value_heads, self.head_dim, self.dtype, self.device)
+            return
+        if attention_type == "Paged_Attn":
+            self.kv_cache = paged_cache(self.num_layers, batch_size, input_length + max_new_length, self.num_key_value_heads,
+                                        self.num_heads, self.head_dim, self.dtype, self.device, **(attn_config or {}))
             return
         if attention_type != "RetroInfer":
             raise ValueError(f"unknown attention type {attention_type}")
@@ -175,6 +181,8 @@ class LlamaModel:
     def decode_attention(self, q, k, v, layer_idx):
         if self.attention_type == "RetroInfer":
             return retroinfer_decode_attn(q, k, v, layer_idx, self.kv_cache)
+        if self.attention_type == "Paged_Attn":
+            return paged_decode_attn(q, k, v, layer_idx, self.kv_cache)
         out = torch.nn.functional.scaled_dot_product_attention(
             q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), enable_gqa=True)
         return out.transpose(1, 2)

@@ -36,7 +36,8 @@ struct PagedAttendParams {
   int64_t sb, sh;         // its strides
   float* part_ml;         // [workgroups + B * heads, GP, 2]: maximum (of scores in units of ln 2) and sum of a part
   float* part_acc;        // [workgroups + B * heads, GP, D]
-  float* logits;          // [B * heads, gs, max_len], units of ln 2
+  int2* shares;           // [B * heads]: the workgroups that have a group's first and its last chunk
+  float* logits;          // [B * heads, max_len, GP], units of ln 2, with scores
   int B, gs, max_len;
   int workgroups;         // that share the rows; 0: one to each group, which writes the output
   float scale2;           // scale / ln 2
@@ -80,6 +81,13 @@ struct PagedRun {
   int64_t from;          // those of one head in front of sequence b's
   int b;
 };
+// sixteen bytes that are read once: a load that leaves the caches to others
+__device__ __forceinline__ uint4 pg_once16(const void* p) {
+  typedef uint32_t words __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(uint4, __builtin_nontemporal_load((const words*)p));
+}
+template <int N>
+struct alignas(4 * N) pg_heads { float x[N]; };
 // x, from which nothing that the compiler knows is to be kept in registers over what stands before
 __device__ __forceinline__ int pg_anew(int x) {
   asm volatile("" : "+v"(x));
@@ -88,15 +96,16 @@ __device__ __forceinline__ int pg_anew(int x) {
 __device__ __forceinline__ int64_t pg_uniform(int64_t x) {
   return (int64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)x) | (int64_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32;
 }
-// Whole workgroup of THREADS: the run, and of the sequences the one for which is_it(b, from, places, each) holds.
-template <int THREADS, typename IsIt>
-__device__ __forceinline__ PagedRun pg_run(const PagedAttendParams& P, IsIt&& is_it) {
+// Whole workgroup: the run, and the sequence that has this workgroup's first place (nothing, where the run is shorter).
+template <int THREADS>
+__device__ __forceinline__ PagedRun pg_run(const PagedAttendParams& P) {
   constexpr int NW = THREADS / 64;
   __shared__ uint32_t sh_wave[NW];
   __shared__ int64_t sh_from;
   __shared__ int sh_b;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const bool one = P.B <= THREADS;
+  const int64_t heads = P.c.heads;
   int64_t sum = 0, each = 0;
   for (int pass = one ? 1 : 0; pass < 2; ++pass) {   // the sum first; of few sequences everything at once
     int64_t in_front = 0;
@@ -115,10 +124,11 @@ __device__ __forceinline__ PagedRun pg_run(const PagedAttendParams& P, IsIt&& is
       }
       if (one) sum = all;
       if (pass) {
-        const int64_t share = (sum * P.c.heads + P.workgroups - 1) / P.workgroups;
+        const int64_t share = (sum * heads + P.workgroups - 1) / P.workgroups;
         each = share < PG_SHARE ? PG_SHARE : share;
-        if (b < P.B && is_it(b, in_front + before, n, each)) {
-          sh_from = in_front + before;
+        const int64_t from = in_front + before, place = blockIdx.x * each;
+        if (from * heads <= place && place < (from + n) * heads) {
+          sh_from = from;
           sh_b = b;
         }
       }
@@ -127,7 +137,7 @@ __device__ __forceinline__ PagedRun pg_run(const PagedAttendParams& P, IsIt&& is
     sum = in_front;
   }
   __syncthreads();
-  return {pg_uniform(each), pg_uniform(sum * P.c.heads), pg_uniform(sh_from), __builtin_amdgcn_readfirstlane(sh_b)};
+  return {pg_uniform(each), pg_uniform(sum * heads), pg_uniform(sh_from), __builtin_amdgcn_readfirstlane(sh_b)};
 }
 
 // s = scale q.k, p = exp(s - m), out = sum p v / sum p over the rows of one (sequence, key-value head), one pass with the running
@@ -150,11 +160,9 @@ __global__ __launch_bounds__(64 * PG_WAVES, UNI && GP < 16 ? 4 : 2) void paged_a
   int b = blockIdx.x / P.c.heads, head = blockIdx.x - b * P.c.heads, skip = 0;   // skip: places of the group that are others'
   int64_t at = 0, end = 0;        // this workgroup's places of the run that are still to be done
   if (P.workgroups) {
-    const int64_t i = blockIdx.x, heads = P.c.heads;
-    const PagedRun run = pg_run<64 * PG_WAVES>(P, [&](int, int64_t from, int places, int64_t each) {
-      return from * heads <= i * each && i * each < (from + places) * heads;
-    });
-    at = i * run.each;
+    const int64_t heads = P.c.heads;
+    const PagedRun run = pg_run<64 * PG_WAVES>(P);
+    at = blockIdx.x * run.each;
     if (at >= run.total) return;
     end = min(at + run.each, run.total);
     b = run.b;
@@ -213,7 +221,10 @@ __global__ __launch_bounds__(64 * PG_WAVES, UNI && GP < 16 ? 4 : 2) void paged_a
     return row < w1 && (unsigned)page < (unsigned)P.c.pages ? page : -1;
   };
   // A chunk's keys and values are requested as soon as the registers of the one before are free, whether their rows are attended
-  // or not (rows of page 0 stand in for those of a page that is not there): no load is under a condition.
+  // or not (rows of page 0 stand in for those of a page that is not there): no load is under a condition.  The values' lines are
+  // read once and whole; told so, the memory gives 6.5 TB/s instead of 5.9 (four sequences of 131072 tokens, 8 heads: 365 -> 330 us;
+  // 32 of 4096 104 -> 95).  The keys' are not: two loads share a line (with them too 332 and 96, sixteen query heads to a head 116
+  // -> 126), nor are those of pages below sixteen rows (110 us either way).
   int cb = c0, pid = units(c0), pid_next = units(c0 + cpb);
   int pk = -1, pv[NV];
   uint4 k[KK], v[NV];
@@ -242,7 +253,7 @@ __global__ __launch_bounds__(64 * PG_WAVES, UNI && GP < 16 ? 4 : 2) void paged_a
     const uint16_t* from = vb + max(pk, 0) * P.c.vp + ((c << 4) & mask) * P.c.vr + voff;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-      v[i] = UNI ? ri_ld16(from + RPI * i * P.c.vr)
+      v[i] = UNI ? pg_once16(from + RPI * i * P.c.vr)
                  : ri_ld16(vb + max(pv[i], 0) * P.c.vp + ((lane / LPR + RPI * i) & mask) * P.c.vr + (lane % LPR) * 8);
   };
   if (c0 < c1) {
@@ -271,13 +282,14 @@ __global__ __launch_bounds__(64 * PG_WAVES, UNI && GP < 16 ? 4 : 2) void paged_a
       load_values(c + 1);
     }
     float al[NH];
+    pg_heads<NH> sv;
     bool rescale = false;
 #pragma unroll
     for (int i = 0; i < NH; ++i) {
       const int r = GP == 16 ? i : rsel + i;
       const float x = r == 0 ? s4[0] : r == 1 ? s4[1] : r == 2 ? s4[2] : s4[3];
       const float s = valid ? x * P.scale2 : -INFINITY;
-      if (P.logits && rk < w1 && head_of(i) < P.gs) P.logits[((size_t)g * P.gs + head_of(i)) * P.max_len + rk] = s;
+      sv.x[i] = s;
       const float mn = fmaxf(m[i], pg_row_max(s));
       const bool none = mn == -INFINITY;   // relative to -inf they would weigh NaN
       al[i] = none ? 1.f : pg_exp2(m[i] - mn);
@@ -287,6 +299,8 @@ __global__ __launch_bounds__(64 * PG_WAVES, UNI && GP < 16 ? 4 : 2) void paged_a
       m[i] = mn;
       pb[head_of(i) * 16 + n] = ri_f32_to_e16<HALF>(p);
     }
+    // (a lane's heads are neighbours, and a chunk's scores one piece of memory)
+    if (P.logits && rk < w1) *reinterpret_cast<pg_heads<NH>*>(P.logits + ((size_t)g * P.max_len + rk) * GP + head_of(0)) = sv;
     const bool any = __builtin_amdgcn_ballot_w64(rescale) != 0;
     if (any && n == 0) {
 #pragma unroll
@@ -330,6 +344,10 @@ __global__ __launch_bounds__(64 * PG_WAVES, UNI && GP < 16 ? 4 : 2) void paged_a
       for (int dt = 0; dt < DT; ++dt) mine[hd * D + 16 * dt + n2] = acc[dt][i];
     }
   }
+  if (P.workgroups && tid == 0) {
+    if (w0 == (first & ~15)) P.shares[g].x = blockIdx.x;
+    if (w1 == last) P.shares[g].y = blockIdx.x;
+  }
   __syncthreads();
   for (int at = tid; at < P.gs * D; at += 64 * PG_WAVES) {
     const int j = at / D, d = at % D;
@@ -365,7 +383,7 @@ __global__ __launch_bounds__(64 * PG_WAVES, UNI && GP < 16 ? 4 : 2) void paged_a
 }
 
 #define PG_JOIN_THREADS 256
-#define PG_JOIN_ROWS (4 * PG_JOIN_THREADS)   // scores of a workgroup of the join, four to a thread
+#define PG_JOIN_ROWS (4 * PG_JOIN_THREADS)   // scores of a workgroup of the join
 #define PG_WORKGROUPS 1024                   // that share the rows at most: parts of a group
 
 // Grid (B * heads, (workgroups ? gs : 0) + ceil(max_len / PG_JOIN_ROWS) with scores): the first gs workgroups of a group join the
@@ -382,16 +400,10 @@ __global__ __launch_bounds__(PG_JOIN_THREADS) void paged_join_kernel(PagedAttend
   const bool joins = (int)blockIdx.y < outs;
   const int r0 = ((int)blockIdx.y - outs) * PG_JOIN_ROWS;
   if (!joins && (r0 >= last || r0 + PG_JOIN_ROWS <= first)) return;
-  int64_t s0 = 0, s1 = first < last;   // the workgroups that have rows of the group
-  if (P.workgroups && first < last) {
-    const PagedRun run = pg_run<PG_JOIN_THREADS>(P, [&](int seq, int64_t, int, int64_t) { return seq == b; });
-    const int places = pg_places(P, b);
-    const int64_t start = run.from * P.c.heads + (int64_t)head * places;
-    s0 = (start + PG_LEAD) / run.each;
-    s1 = (start + places - 1) / run.each + 1;
-  }
-  const int parts = (int)(s1 - s0);
-  const size_t part0 = (size_t)(g + s0);
+  // the group's parts: of each workgroup that has rows of it
+  const int2 share = P.workgroups && first < last ? P.shares[g] : make_int2(0, first < last ? 0 : -1);
+  const int parts = share.y - share.x + 1;
+  const size_t part0 = (size_t)g + share.x;
   const float2* const ml = reinterpret_cast<const float2*>(P.part_ml) + part0 * GP;
   // maximum and sum of a head's parts, by a wave
   const auto join = [&](int j) {
@@ -446,37 +458,30 @@ __global__ __launch_bounds__(PG_JOIN_THREADS) void paged_join_kernel(PagedAttend
     if (threadIdx.x == 0 && P.lse) P.lse[o] = L == 0.f ? -INFINITY : (M + __log2f(L)) * PG_LN2;
     return;
   }
-  const int r = r0 + 4 * threadIdx.x;
-  float* const scores = P.scores + b * P.sb + head * P.sh + r;
-  const float* const logits = P.logits + (size_t)g * P.gs * P.max_len + r;
-  const bool whole = r >= first && r + 4 <= last;
-  pg_f4 x[GP], was;
-  if (whole) {
-    was = *reinterpret_cast<const pg_f4*>(scores);
+  // rows r0 + threadIdx.x + 256 i
+  float* const scores = P.scores + b * P.sb + head * P.sh;
+  pg_heads<GP> x[4];
+  float was[4];
 #pragma unroll
-    for (int j = 0; j < GP; ++j) x[j] = *reinterpret_cast<const pg_f4*>(logits + (size_t)min(j, P.gs - 1) * P.max_len);
+  for (int i = 0; i < 4; ++i) {
+    const int r = min(max(r0 + (int)threadIdx.x + PG_JOIN_THREADS * i, first), last - 1);
+    x[i] = *reinterpret_cast<const pg_heads<GP>*>(P.logits + ((size_t)g * P.max_len + r) * GP);
+    was[i] = scores[r];
   }
   for (int j = wave; j < P.gs; j += NW) join(j);
   __syncthreads();
-  if (whole) {
 #pragma unroll
-    for (int j = 0; j < GP; ++j) {
-      const float M = sh_M[min(j, P.gs - 1)], L = sh_L[min(j, P.gs - 1)], inv = j < P.gs && L != 0.f ? 1.f / L : 0.f;
-      if (inv != 0.f)
+  for (int j = 0; j < GP; ++j) {
+    const float M = sh_M[min(j, P.gs - 1)], L = sh_L[min(j, P.gs - 1)];
+    if (j >= P.gs || L == 0.f) continue;   // (no rows: nothing to add)
+    const float inv = 1.f / L;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) was[i] += pg_exp2(x[j][i] - M) * inv;
-    }
-    *reinterpret_cast<pg_f4*>(scores) = was;
-  } else {
-    for (int i = 0; i < 4; ++i) {
-      if (r + i < first || r + i >= last) continue;
-      float w = scores[i];
-      for (int j = 0; j < P.gs; ++j) {
-        const float L = sh_L[j], inv = L != 0.f ? 1.f / L : 0.f;
-        if (inv != 0.f) w += pg_exp2(logits[(size_t)j * P.max_len + i] - sh_M[j]) * inv;
-      }
-      scores[i] = w;
-    }
+    for (int i = 0; i < 4; ++i) was[i] += pg_exp2(x[i].x[j] - M) * inv;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = r0 + threadIdx.x + PG_JOIN_THREADS * i;
+    if (r >= first && r < last) scores[r] = was[i];
   }
 }
 
@@ -916,7 +921,8 @@ extern "C" size_t ri_paged_attention_workspace_bytes(int B, int heads, int gs, i
   if (B <= 0 || heads <= 0 || gs <= 0 || gs > 16 || max_len <= 0 || max_len > PG_MAX_ROWS || (dim != 64 && dim != 128)) return 0;
   const int64_t groups = (int64_t)B * heads;
   const size_t parts = groups + paged_workgroups(groups, max_len);
-  return parts * pg_pad(gs) * (2 + dim) * sizeof(float) + (scored ? (size_t)groups * gs * max_len * sizeof(float) : 0);
+  return parts * pg_pad(gs) * (2 + dim) * sizeof(float) + (scored ? (size_t)groups * pg_pad(gs) * max_len * sizeof(float) : 0) +
+         groups * sizeof(int2);
 }
 
 template <int D, int GP, bool HALF>
@@ -965,6 +971,7 @@ extern "C" int ri_paged_attention(const ri_paged_t* cache, const void* q, const 
   P.part_ml = (float*)workspace;
   P.part_acc = P.part_ml + 2 * parts;
   P.logits = scores ? P.part_acc + parts * cache->dim : nullptr;
+  P.shares = (int2*)(P.part_acc + parts * cache->dim + (scores ? (size_t)groups * pg_pad(gs) * max_len : 0));
   hipStream_t s = (hipStream_t)stream;
   if (cache->dim == 64) cache->half ? launch_paged_gp<64, true>(P, groups, s) : launch_paged_gp<64, false>(P, groups, s);
   else cache->half ? launch_paged_gp<128, true>(P, groups, s) : launch_paged_gp<128, false>(P, groups, s);

@@ -98,7 +98,7 @@ __device__ __forceinline__ int weigh_last_key(const WeighParams& P, int n, int s
   return n - P.W + min((super + 1) * P.per * block - 1, P.cols - 1) / P.gs;
 }
 
-// One pass over the keys [j0, j1) of split blockIdx.z of group blockIdx.x, of which the columns [32 wave, 32 wave + 32) of
+// One pass over the keys [j0, j1) of a split of group blockIdx.x, of which the columns [32 wave, 32 wave + 32) of
 // a block of 32 WAVES see some.
 // SUM false: the lse, of a block's columns as columns of the product;
 // m and l of a lane: its reference and the sum of exponentials relative to it, over its own keys.  The reference is the maximum of
@@ -119,7 +119,9 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void weigh_kernel(WeighParams P) {
   const int blocks = (P.cols + BLOCK - 1) / BLOCK;
   const int super = gridDim.y - 1 - blockIdx.y;                     // (the columns that see most keys first)
   const int block0 = SUM ? super * P.per : super, block1 = SUM ? min(block0 + P.per, blocks) : block0 + 1;
-  const int j0 = blockIdx.z * P.rows, jn = min(j0 + P.rows, n);
+  // (the second pass begins with the keys that the first ended with, which the memory-side cache may still hold)
+  const int split = SUM ? gridDim.z - 1 - blockIdx.z : blockIdx.z;
+  const int j0 = split * P.rows, jn = min(j0 + P.rows, n);
   const uint16_t* const keys = P.key + b * P.kb + head * P.kh;
   uint32_t at[LOADS];   // of this lane's piece of a tile's rows
 #pragma unroll
@@ -311,7 +313,7 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void weigh_kernel(WeighParams P) {
   const float Z = ri_xor_sum<32>(m == -INFINITY ? l : l * __builtin_amdgcn_exp2f(m - M));
   if (lane < 32) {
     const int col = block0 * BLOCK + wave * 32 + lane;
-    float* const to = P.stats + (((size_t)g * P.S + blockIdx.z) * P.cols_pad + col) * 2;
+    float* const to = P.stats + (((size_t)g * P.S + split) * P.cols_pad + col) * 2;
     to[0] = col < P.cols ? M : -INFINITY;
     to[1] = col < P.cols ? Z : 0.f;
   }

@@ -670,7 +670,8 @@ int ri_prefill_index_f16(const void* centroids, const void* mean, const int32_t*
  * k_pages + p * k_page_stride + h * k_head_stride on, k_row_stride apart (elements; multiples of 8, the base 16-byte aligned), and so
  * do the values.  Row r of sequence b is row r % page_rows of page block_table[b * table_stride + r / page_rows]; an entry outside
  * [0, pages) is a page that is not there: its rows are neither attended nor written.  dim 64 or 128, page_rows a power of two, at
- * most 2^24 rows to a sequence.  half: IEEE half instead of bfloat16. */
+ * most 2^24 rows to a sequence.  half: IEEE half instead of bfloat16.  Sequences may share pages that are only read; a page that
+ * ri_paged_append or ri_paged_fill writes belongs to one sequence of the call. */
 typedef struct ri_paged_t {
   void* k_pages;
   void* v_pages;

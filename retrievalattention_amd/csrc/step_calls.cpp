@@ -553,7 +553,7 @@ PyObject* attention_weights(PyObject*, PyObject* const* args, Py_ssize_t n) {
     Py_RETURN_NONE;
   const int gs = (int)(hq / heads);
   const size_t bytes = ri_attention_weights_workspace_bytes((int)B, (int)heads, gs, (int)W, (int)T);
-  void* const ws = paged_scratch(args[4], bytes, device);
+  void* const ws = bytes ? paged_scratch(args[4], bytes, device) : nullptr;
   if (!ws) Py_RETURN_NONE;
   at::Tensor out = at::empty({B, heads, T}, key->options().dtype(at::kFloat).requires_grad(false));
   void *qp = q->data_ptr(), *kp = key->data_ptr(), *np = address(lens), *op = out.data_ptr();

@@ -32,10 +32,11 @@ struct WeighParams {
   float* out;             // [B, heads, T]
   float* stats;           // [B * heads, S, cols_pad, 2] maximum (units of ln 2) and sum of the splits
   float* lse;             // [B * heads, cols_pad], units of ln 2; +inf: the column has no keys
-  float* part;            // [B * heads, supers, T] sums of `per` blocks of columns each
+  float* part;            // [B * heads, supers, T] their sums
   int heads, gs, W, T, cols, cols_pad;
-  int S, rows;            // splits of the keys, keys of one
-  int per, supers;
+  int S;                  // splits of the keys in the first pass
+  int rows;               // keys of a split of the pass
+  int per, supers;        // blocks of columns to a workgroup of the second pass, workgroups to all
   int joined;             // whether lse is filled before the second kernel
   float scale2;           // scale / ln 2
 };
@@ -347,41 +348,53 @@ __global__ __launch_bounds__(256) void weigh_add_kernel(WeighParams P) {
 }
 
 // ------------------------------------------------------------------------------------ host side
-struct WeighPlan { int cols_pad, S, rows, per, supers; bool joined; };
+struct WeighPlan { int cols_pad, S, rows, S2, rows2, per, supers; bool joined, wide; };
 static int weigh_up(int64_t n, int to) { return (int)((n + to - 1) / to * to); }
-// Keys of a split: as many workgroups of the first pass as fit the compute units at a time, two to each, and no more keys than
-// the second has LDS for.  The second pass takes one block of columns to a workgroup, whose sums are a part of the result (8192
-// queries and keys, 32 heads: parts of 67 MB), and more of them, which it adds up in LDS, where the parts would pass 256 MB.
-// Two blocks over few keys are one workgroup's too (a launch less: 224 columns, 1111 keys, 4 heads 21.6 -> 17.4 us; up to 448 keys
-// LDS still holds three workgroups, of more it costs more than the launch).  Up to sixteen splits are joined by whoever needs them,
-// more by a launch of their own.
+// Keys of a split: as many workgroups as fit the compute units at a time, two to each in the first pass and three in the second.
+// The second pass takes one block of columns to a workgroup, whose sums are a part of the result (8192 queries and keys, 32 heads:
+// parts of 67 MB), and more of them, which it adds up in LDS, where the parts would pass 256 MB.  Two blocks over few keys are one
+// workgroup's of twice the waves (`wide`): they need not be added up by a launch of their own, and there are compute units enough
+// (224 columns, 1111 keys, 4 heads: the pass and the launch 6.3 + 2.8 us, two blocks in turn 10.9, wide 7.7).  Up to sixteen splits are
+// joined by whoever needs them, more by a launch of their own.
 static WeighPlan weigh_plan(int64_t groups, int cols, int T) {
   WeighPlan p;
   p.cols_pad = weigh_up(cols, WG_COLS);
-  const int64_t want = (T * groups * (p.cols_pad / WG_COLS) + 511) / 512;
-  p.rows = weigh_up(want < 128 ? 128 : want > WG_ROWS ? WG_ROWS : want, WG_TILE);
-  p.S = (T + p.rows - 1) / p.rows;
+  const auto split = [&](int64_t workgroups, int at_a_time, int most, int* rows, int* S) {
+    const int64_t want = (T * workgroups + at_a_time - 1) / at_a_time;
+    *rows = weigh_up(want < 128 ? 128 : want > most ? most : want, WG_TILE);
+    *S = (T + *rows - 1) / *rows;
+  };
+  split(groups * (p.cols_pad / WG_COLS), 512, WG_ROWS, &p.rows, &p.S);
   const int64_t blocks = weigh_up(cols, WG_SUM_COLS) / WG_SUM_COLS;
   const int64_t per = (groups * blocks * T * (int64_t)sizeof(float) + (1 << 28) - 1) >> 28;
-  p.per = (int)(per < blocks ? per : blocks);
-  if (blocks == 2 && p.rows <= 448) p.per = 2;
-  p.supers = (int)((blocks + p.per - 1) / p.per);
+  p.wide = blocks == 2 && groups * ((T + 127) / 128) <= 256;
+  p.per = p.wide ? 1 : (int)(per < blocks ? per : blocks);
+  p.supers = p.wide ? 1 : (int)((blocks + p.per - 1) / p.per);
+  split(groups * p.supers, p.wide ? 256 : 768, WG_ROWS, &p.rows2, &p.S2);
   p.joined = p.S > 16;
   return p;
 }
 
 extern "C" size_t ri_attention_weights_workspace_bytes(int B, int heads, int gs, int W, int T) {
-  if (B <= 0 || heads <= 0 || gs <= 0 || gs > 16 || W <= 0 || T < W || T > 1 << 24 || (int64_t)B * heads > 65535) return 0;
+  if (B <= 0 || heads <= 0 || gs <= 0 || gs > 16 || W <= 0 || T < W || T > 1 << 24 || (int64_t)B * heads > 65535 ||
+      (int64_t)W * gs > (int64_t)65535 * WG_SUM_COLS)   // (dimensions of grids)
+    return 0;
   const WeighPlan p = weigh_plan((int64_t)B * heads, W * gs, T);
   return (size_t)B * heads * ((size_t)p.cols_pad * (2 * (size_t)p.S + (p.joined ? 1 : 0)) + (p.supers > 1 ? (size_t)p.supers * T : 0)) * sizeof(float);
 }
 
 template <int D, bool HALF>
-static void launch_weigh(const WeighParams& P, int groups, hipStream_t s) {
-  weigh_kernel<D, HALF, false, WG_COLS / 32, 4><<<dim3(groups, P.cols_pad / WG_COLS, P.S), 2 * WG_COLS, 0, s>>>(P);
+static void launch_weigh(WeighParams P, const WeighPlan& p, int groups, hipStream_t s) {
+  weigh_kernel<D, HALF, false, WG_COLS / 32, 4><<<dim3(groups, P.cols_pad / WG_COLS, p.S), 2 * WG_COLS, 0, s>>>(P);
   if (P.joined) weigh_join_kernel<<<dim3(P.cols_pad / 32, groups), 256, 0, s>>>(P);
-  weigh_kernel<D, HALF, true, WG_SUM_COLS / 32, 3><<<dim3(groups, P.supers, P.S), 2 * WG_SUM_COLS, P.per > 1 ? P.rows * sizeof(float) : 0, s>>>(P);
-  if (P.supers > 1) weigh_add_kernel<<<dim3((P.T + 255) / 256, groups), 256, 0, s>>>(P);
+  P.rows = p.rows2;
+  const dim3 grid(groups, p.supers, p.S2);
+  if (p.wide) {
+    weigh_kernel<D, HALF, true, WG_COLS / 32, 2><<<grid, 2 * WG_COLS, 0, s>>>(P);
+  } else {
+    weigh_kernel<D, HALF, true, WG_SUM_COLS / 32, 3><<<grid, 2 * WG_SUM_COLS, P.per > 1 ? P.rows * sizeof(float) : 0, s>>>(P);
+    if (P.supers > 1) weigh_add_kernel<<<dim3((P.T + 255) / 256, groups), 256, 0, s>>>(P);
+  }
 }
 
 static int attention_weights_impl(const void* q, const void* key, const int32_t* seqlens, float* out, int64_t q_batch_stride,
@@ -404,8 +417,8 @@ static int attention_weights_impl(const void* q, const void* key, const int32_t*
                          lse + (p.joined ? (size_t)groups * p.cols_pad : 0), heads, gs, W, T, cols, p.cols_pad, p.S, p.rows, p.per,
                          p.supers, p.joined, scale * WG_LOG2E};
   hipStream_t s = (hipStream_t)stream;
-  if (dim == 64) half ? launch_weigh<64, true>(P, groups, s) : launch_weigh<64, false>(P, groups, s);
-  else half ? launch_weigh<128, true>(P, groups, s) : launch_weigh<128, false>(P, groups, s);
+  if (dim == 64) half ? launch_weigh<64, true>(P, p, groups, s) : launch_weigh<64, false>(P, p, groups, s);
+  else half ? launch_weigh<128, true>(P, p, groups, s) : launch_weigh<128, false>(P, p, groups, s);
   RI_HIP_CHECK_LAUNCH();
   return RI_OK;
 }

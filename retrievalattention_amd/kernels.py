@@ -900,8 +900,8 @@ def _paged(k_pages, v_pages, block_table, B, writes=False):
 def paged_attention(q, k_pages, v_pages, block_table, cache_seqlens, starts=None, scores=None, scale=None,
                     return_softmax_lse=False, max_len=None, scratch=None):
     """Attention of one new token of each sequence over the rows of its pages (the token's own appended before).
-    q [B, 1, heads * gs, dim]; k_pages, v_pages [pages, heads, page_rows, dim] (strided or not, page_rows a power of two, dim 64 or
-    128); block_table [B, n] int32, the pages of a sequence in order; cache_seqlens [B] int32, the rows in use.  An entry of the
+    q [B, 1, heads * gs, dim] contiguous; k_pages, v_pages [pages, heads, page_rows, dim] (strided or not, page_rows a power of two,
+    dim 64 or 128); block_table [B, n] int32, the pages of a sequence in order; cache_seqlens [B] int32, the rows in use.  An entry of the
     table that is no page of the pool stands for rows that are not there.  starts [B] int32: the first row that is attended.
     scores [B, heads, rows] fp32: each row's weights, summed over the gs query heads of its head, are added to it.
     max_len: no sequence has more rows (default: what the table holds; rows from max_len on are not attended), which sizes the
@@ -946,7 +946,8 @@ def paged_append(key, value, k_pages, v_pages, block_table, cache_seqlens, new_s
     the table holds) takes them as its next row; in a full one, given `scores` [B, heads, rows] fp32, `positions` [B, heads, rows]
     int32 and `token_positions` [B] int32 (the token's place in its sequence), they take the place of the row with the lowest score
     in each head, the first `sinks` and the last `recent` tokens of the sequence (the new one is the last) excepted; equal scores:
-    the lowest row.  The row's score becomes 0, its position the token's.  A full sequence without scores is left as it is.
+    the lowest row; a NaN counts as the highest.  The row's score becomes 0, its position the token's.  A full sequence without
+    scores is left as it is.  The page that takes the row must be no other sequence's.
     new_seqlens [B] int32, another tensor than cache_seqlens: the rows in use afterwards."""
     status = step_calls().paged_append(key, value, k_pages, v_pages, block_table, cache_seqlens, new_seqlens, scores, positions,
                                        token_positions, budget, sinks, recent)
@@ -987,7 +988,7 @@ def paged_fill(key, value, k_pages, v_pages, block_table, new_seqlens=None, seql
     T).  Of a prompt of more than `budget` tokens (default: the rows that the table holds) each head keeps `budget`: the first
     `sinks`, the last `recent` and of the others those with the highest weights [B, heads, T] fp32 (attention_weights), at equal
     weights the first ones, in their order.  new_seqlens [B] int32: the rows written.  scores, positions [B, heads, rows]: take the
-    kept weights and the tokens' places."""
+    kept weights and the tokens' places.  A sequence's pages must be no other's."""
     status = step_calls().paged_fill(key, value, k_pages, v_pages, block_table, new_seqlens, seqlens, weights, scores, positions,
                                      budget, sinks, recent, _held(key, "paged_fill", scratch))
     if status is not None:
@@ -1038,7 +1039,7 @@ def attention_weights(q, key, seqlens=None, scale=None, scratch=None):
     B, W, hq, dim = q.shape
     T, heads = key.shape[1:3]
     if key.shape[0] != B or key.shape[3] != dim or dim not in PAGED_DIMS or not 1 <= W <= T <= 1 << 24 or B < 1 or heads < 1 or \
-            hq % heads or not 1 <= hq // heads <= MAX_GROUP_SIZE or B * heads > 65535:
+            hq % heads or not 1 <= hq // heads <= MAX_GROUP_SIZE or B * heads > 65535 or W * (hq // heads) > 65535 * 128:
         raise ValueError("attention_weights: expected q [B, W <= T, heads * 1 .. 16, dim] and key [B, T, heads, 64 or 128]")
     qs, ks = _strided(q, 4, key.dtype, key.device, "q"), _strided(key, 4, key.dtype, key.device, "key")
     if seqlens is not None:

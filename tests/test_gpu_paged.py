@@ -392,3 +392,78 @@ def test_prompt_weights_far_apart(dev):
     # (each score is exact up to a rounding of its sum and one of its product with 1 / ln 2: 3 roundings of 3600 / ln 2 here)
     rel = 8 * F * (1 + size) * 1.5 + 64 * F
     assert bool(((got - want).abs() <= rel * want + 1e-30).all())
+
+
+def test_native_and_general_calls_do_the_same(dev, monkeypatch):
+    """The native calls launch what the wrappers' general way launches; arguments that are not in order reach the general way,
+    which words the error."""
+    gen = torch.Generator().manual_seed(12)
+    B, heads, gs, dim, page, T, budget = 3, 2, 4, 64, 16, 200, 40
+    k, v, table = _pool(gen, HF, B, heads, dim, page, budget, junk=False)
+    key, q = _randn(gen, B, T, heads, dim).to(HF).to(dev), _randn(gen, B, T, heads * gs, dim).to(HF).to(dev)
+    lens = torch.tensor([200, 40, 17], dtype=torch.int32, device=dev)
+
+    class General:
+        def __getattr__(self, name):
+            return lambda *a: None
+
+    def run():
+        kk, vv, held, more = k.to(dev), v.to(dev), torch.zeros(B, dtype=torch.int32, device=dev), torch.zeros(B, dtype=torch.int32, device=dev)
+        scores = torch.zeros(B, heads, budget, device=dev)
+        positions = torch.zeros(B, heads, budget, dtype=torch.int32, device=dev)
+        t = table.to(dev)
+        w = kernels.attention_weights(q[:, -9:], key, seqlens=lens, scale=0.1)
+        kernels.paged_fill(key, key * 2, kk, vv, t, held, seqlens=lens, weights=w, scores=scores, positions=positions, budget=budget,
+                           sinks=1, recent=3)
+        kernels.paged_append(key[:, :1], key[:, 1:2], kk, vv, t, held, more, scores=scores, positions=positions, token_positions=lens,
+                             budget=budget, sinks=1, recent=3)
+        out, lse = kernels.paged_attention(q[:, :1].contiguous(), kk, vv, t, more, scores=scores, max_len=budget, return_softmax_lse=True)
+        return w, kk, vv, held, more, scores, positions, out, lse
+    first = run()      # (sizes the scratch)
+    native = run()
+    with monkeypatch.context() as m:
+        m.setattr(kernels, "step_calls", General)
+        general = run()
+    for a, b, c in zip(first, native, general):
+        assert torch.equal(a, b) and torch.equal(b, c)
+    w, kk, vv, held, more, scores, positions, _, _ = native
+    odd = torch.zeros(B, T, heads, dim + 8, dtype=HF, device=dev)[..., 1:dim + 1]
+    t = table.to(dev)
+    one = q[:, :1].contiguous()
+    for error, match, call in (
+            (ValueError, "contiguous", lambda: kernels.paged_attention(q[:, :1, :, :].transpose(1, 2).contiguous().transpose(1, 2)[..., ::2], kk, vv, t, more)),
+            (TypeError, "int32", lambda: kernels.paged_attention(one, kk, vv, t, more.long())),
+            (ValueError, "max_len", lambda: kernels.paged_attention(one, kk, vv, t, more, max_len=49)),
+            (ValueError, "scores", lambda: kernels.paged_attention(one, kk, vv, t, more, scores=scores)),   # (48 rows, scores of 40)
+            (ValueError, "query heads", lambda: kernels.paged_attention(one[:, :, :7].contiguous(), kk, vv, t, more)),
+            (ValueError, "cpu|cuda", lambda: kernels.paged_attention(one, kk, vv, table, more)),
+            (TypeError, "float16", lambda: kernels.paged_attention(one.bfloat16(), kk, vv, t, more)),
+            (ValueError, "another tensor", lambda: kernels.paged_append(key[:, :1], key[:, :1], kk, vv, t, held, held)),
+            (ValueError, "budget", lambda: kernels.paged_append(key[:, :1], key[:, :1], kk, vv, t, held, budget=49)),
+            (ValueError, "positions", lambda: kernels.paged_append(key[:, :1], key[:, :1], kk, vv, t, held, scores=scores, budget=40)),
+            (ValueError, "share memory", lambda: kernels.paged_append(key[:, :1], key[:, :1], kk[:1].expand(kk.shape), vv, t, held)),
+            (ValueError, "share memory", lambda: kernels.paged_attention(one, kk, vv, t, more, scores=scores[:1].expand(B, heads, 40), max_len=40)),
+            (ValueError, "weights", lambda: kernels.paged_fill(key, key, kk, vv, t, held, budget=40)),
+            (ValueError, "aligned", lambda: kernels.paged_fill(odd, odd, kk, vv, t, held, weights=w, budget=40)),
+            (ValueError, "W <= T", lambda: kernels.attention_weights(q, key[:, :9])),
+            (RuntimeError, "Half and BFloat16", lambda: kernels.attention_weights(q.float(), key.float()))):
+        with pytest.raises(error, match=match):
+            call()
+
+
+def test_scratch_does_not_grow_in_a_capture(dev):
+    gen = torch.Generator().manual_seed(13)
+    k, v, table = _pool(gen, BF, 1, 1, 64, 16, 64, junk=False)
+    args = [t.to(dev) for t in (_randn(gen, 1, 1, 4, 64).to(BF), k, v, table, torch.tensor([50], dtype=torch.int32))]
+    own = kernels.Scratch()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="capture"), torch.cuda.graph(graph):
+        kernels.paged_attention(*args, scratch=own)
+    want = kernels.paged_attention(*args, scratch=own)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = kernels.paged_attention(*args, scratch=own)
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        assert torch.equal(out, want)

@@ -178,7 +178,6 @@ __global__ __launch_bounds__(64 * PG_WAVES, UNI && GP < 16 ? 4 : 2) void paged_a
   if ((threadIdx.x & 63) < 16) al_sh[threadIdx.x & 63] = 1.f;
   const int shift = P.c.shift, mask = P.c.mask;
   const int upc = UNI ? 1 : 16 >> shift;      // units, of which a lane holds the page, to a chunk
-  const int ush = UNI ? 4 : shift;            // rows of a unit as a power of two
   const int cpb = 64 / upc;                   // chunks to a batch of 64 units
 
   for (;;) {   // the groups that this workgroup has rows of
@@ -208,40 +207,41 @@ __global__ __launch_bounds__(64 * PG_WAVES, UNI && GP < 16 ? 4 : 2) void paged_a
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) acc[dt] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
 
-  // this wave's chunks [c0, c1) of 16 rows
-  const int chunks = (w1 - w0 + 15) >> 4, per = (max(chunks, 0) + PG_WAVES - 1) / PG_WAVES;
-  const int c0 = (w0 >> 4) + min(chunks, wave * per), c1 = min(c0 + per, (w0 >> 4) + chunks);
+  // this wave's chunks of 16 rows: c0, c0 + PG_WAVES, ... below c1 (a run to each wave: 329 instead of 323 us of four sequences of
+  // 131072 tokens, 51 instead of 49 of sixteen of unequal lengths)
+  const int c0 = (w0 >> 4) + wave, c1 = (w1 + 15) >> 4;
   const int32_t* const table = P.c.table + b * P.c.ts;
   const uint16_t* const kb = P.c.k + head * P.c.kh;
   const uint16_t* const vb = P.c.v + head * P.c.vh;
   // the page of this lane's unit of the batch that begins with chunk c; -1 where there is none
   const auto units = [&](int c) {
-    const int row = (c * upc + lane) << ush;
+    const int row = ((c + (UNI ? lane : lane / upc) * PG_WAVES) << 4) + (UNI ? 0 : (lane % upc) << shift);
     const int page = table[min(row >> shift, P.c.table_pages - 1)];
-    return row < w1 && (unsigned)page < (unsigned)P.c.pages ? page : -1;
+    return (unsigned)page < (unsigned)P.c.pages ? page : -1;
   };
   // A chunk's keys and values are requested as soon as the registers of the one before are free, whether their rows are attended
   // or not (rows of page 0 stand in for those of a page that is not there): no load is under a condition.  The values' lines are
   // read once and whole; told so, the memory gives 6.5 TB/s instead of 5.9 (four sequences of 131072 tokens, 8 heads: 365 -> 330 us;
   // 32 of 4096 104 -> 95).  The keys' are not: two loads share a line (with them too 332 and 96, sixteen query heads to a head 116
   // -> 126), nor are those of pages below sixteen rows (110 us either way).
-  int cb = c0, pid = units(c0), pid_next = units(c0 + cpb);
+  int ib = 0, pid = units(c0), pid_next = units(c0 + cpb * PG_WAVES);   // ib: the chunk's place in its batch
   int pk = -1, pv[NV];
   uint4 k[KK], v[NV];
   const uint32_t koff = (uint32_t)n * (uint32_t)P.c.kr + h * 8, voff = (uint32_t)(lane / LPR) * (uint32_t)P.c.vr + (lane % LPR) * 8;
   const auto pages = [&](int c) {
-    if (c == cb + cpb) {
-      cb = c;
+    if (ib == cpb) {
+      ib = 0;
       pid = pid_next;
-      pid_next = units(c + cpb);
+      pid_next = units(c + cpb * PG_WAVES);
     }
     if (UNI) {
-      pk = __builtin_amdgcn_readlane(pid, c - cb);
+      pk = __builtin_amdgcn_readlane(pid, ib);
     } else {
-      pk = __shfl(pid, (c - cb) * upc + (n >> shift));
+      pk = __shfl(pid, ib * upc + (n >> shift));
 #pragma unroll
-      for (int i = 0; i < NV; ++i) pv[i] = __shfl(pid, (c - cb) * upc + ((lane / LPR + RPI * i) >> shift));
+      for (int i = 0; i < NV; ++i) pv[i] = __shfl(pid, ib * upc + ((lane / LPR + RPI * i) >> shift));
     }
+    ++ib;
   };
   const auto load_keys = [&](int c) {
     const uint16_t* from = UNI ? kb + max(pk, 0) * P.c.kp + ((c << 4) & mask) * P.c.kr + koff
@@ -261,7 +261,7 @@ __global__ __launch_bounds__(64 * PG_WAVES, UNI && GP < 16 ? 4 : 2) void paged_a
     load_keys(c0);
     load_values(c0);
   }
-  for (int c = c0; c < c1; ++c) {
+  for (int c = c0; c < c1; c += PG_WAVES) {
     const int r0 = c << 4, rk = r0 + n;
     const bool valid = pk >= 0 && rk >= first && rk < last;
     f32x4_t s4 = (f32x4_t){0.f, 0.f, 0.f, 0.f};
@@ -276,10 +276,10 @@ __global__ __launch_bounds__(64 * PG_WAVES, UNI && GP < 16 ? 4 : 2) void paged_a
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) *reinterpret_cast<uint4*>(vt + (lane / LPR + RPI * i) * VS + (lane % LPR) * 8) = v[i];
-    if (c + 1 < c1) {
-      pages(c + 1);
-      load_keys(c + 1);
-      load_values(c + 1);
+    if (c + PG_WAVES < c1) {
+      pages(c + PG_WAVES);
+      load_keys(c + PG_WAVES);
+      load_values(c + PG_WAVES);
     }
     float al[NH];
     pg_heads<NH> sv;
@@ -607,31 +607,30 @@ __device__ __forceinline__ int pg_prompt(const PagedFillParams& P, int b) { retu
 
 #define PG_SEL_THREADS 1024
 #define PG_SEL_WAVES (PG_SEL_THREADS / 64)
-#define PG_CHUNK (4 * PG_SEL_THREADS)   // rows of a workgroup: four consecutive ones to a thread
+#define PG_CHUNK (4 * PG_SEL_THREADS)   // rows: four consecutive ones to a thread
+#define PG_SEL_CHUNKS 4                 // that one workgroup selects from
 
 // The rows of a prompt that are kept, in order, with their weights and positions: the `sinks` first, the `recent` last and of the
 // others those with the highest weights, at equal weights the first ones.  A radix selection finds the lowest kept order, digits of
 // 11, 11 and 10 bits, and how many of the rows of that order are kept, the first ones.
 struct PagedRows {   // this thread's rows of a chunk
   int r0;
-  uint32_t o[4];     // their orders; none is 0
-  float w[4];
+  uint32_t o[4];     // their orders; 0: no row
 };
 __device__ __forceinline__ PagedRows pg_rows(const PagedFillParams& P, const float* w, int n, int chunk) {
   PagedRows x;
   x.r0 = chunk * PG_CHUNK + 4 * threadIdx.x;
+  pg_f4 v = {0.f, 0.f, 0.f, 0.f};
   if (x.r0 + 4 <= n) {
-    const pg_f4 v = *reinterpret_cast<const pg_f4*>(w + x.r0);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x.w[i] = v[i];
+    v = *reinterpret_cast<const pg_f4*>(w + x.r0);
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x.w[i] = x.r0 + i < n ? w[x.r0 + i] : 0.f;
+    for (int i = 0; i < 4; ++i) v[i] = x.r0 + i < n ? w[x.r0 + i] : 0.f;
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int r = x.r0 + i;
-    x.o[i] = r >= n ? 0u : r < P.sinks || r >= n - P.recent ? 0xffffffffu : pg_order(x.w[i]);
+    x.o[i] = r >= n ? 0u : r < P.sinks || r >= n - P.recent ? 0xffffffffu : pg_order(v[i]);
   }
   return x;
 }
@@ -680,9 +679,9 @@ __device__ __forceinline__ uint32_t pg_scan(uint32_t x, uint32_t* all) {
 }
 
 // This thread's rows of order above `lowest`, and the first `need` of those of it, to their places: `base` rows and `ties` of that
-// order are in front of the chunk's.
+// order are in front of the chunk's, and behind it when this returns.
 __device__ __forceinline__ void pg_emit(const PagedFillParams& P, int g, int b, int head, const PagedRows& x, uint32_t lowest, int need,
-                                        int base, int ties) {
+                                        int& base, int& ties) {
   uint32_t mine = 0, all;
 #pragma unroll
   for (int i = 0; i < 4; ++i) mine += (x.o[i] > lowest ? 1u : 0u) + (x.o[i] == lowest ? 0x10000u : 0u);
@@ -691,18 +690,22 @@ __device__ __forceinline__ void pg_emit(const PagedFillParams& P, int g, int b, 
   int32_t* const kept = P.kept + (size_t)g * P.budget;
   float* const scores = P.scores ? P.scores + b * P.sb + head * P.sh : nullptr;
   int32_t* const positions = P.positions ? P.positions + b * P.pb + head * P.ph : nullptr;
+  const float* const w = P.weights + b * P.wb + head * P.wh;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const bool is_above = x.o[i] > lowest, is_tie = x.o[i] == lowest;
     if (is_above || (is_tie && tie < need)) {
       const int at = base + above + min(tie, need) - min(ties, need);
       kept[at] = x.r0 + i;
-      if (scores) scores[at] = x.w[i];
+      if (scores) scores[at] = w[x.r0 + i];
       if (positions) positions[at] = x.r0 + i;
     }
     above += is_above;
     tie += is_tie;
   }
+  const int more = (int)(all >> 16);
+  base += (int)(all & 0xffffu) + min(ties + more, need) - min(ties, need);
+  ties += more;
 }
 
 // Scores and positions of the rows [r0, r1) of a prompt that is kept whole.
@@ -716,29 +719,39 @@ __device__ __forceinline__ void pg_whole(const PagedFillParams& P, int b, int he
   }
 }
 
-// Grid (heads, B): prompts of one chunk at most, and longer ones that are kept whole (ALL).
-template <bool ALL>
+// Grid (heads, B): a workgroup has a prompt of up to CHUNKS chunks, whose orders stay in registers (0: prompts that are kept whole).
+// A prompt of 6000 tokens, 16 (sequence, head) pairs, with the copy: 11.9 us against 20 in launches over chunks, 12000: 15.7 and 20.1;
+// with eight chunks it loses, 30011: 30.7 and 21.7.
+template <int CHUNKS>
 __global__ __launch_bounds__(PG_SEL_THREADS) void paged_select_kernel(PagedFillParams P) {
   __shared__ int hist[2048];
   const int head = blockIdx.x, b = blockIdx.y, n = pg_prompt(P, b), g = b * P.c.heads + head;
   if (n <= P.budget) return pg_whole(P, b, head, 0, n);
-  if (ALL) return;
-  const PagedRows x = pg_rows(P, P.weights + b * P.wb + head * P.wh, n, 0);
-  uint32_t lowest = 0, known = 0;   // bits of the lowest kept order found so far
-  int need = P.budget;
+  if constexpr (CHUNKS > 0) {
+    PagedRows x[CHUNKS];
 #pragma unroll
-  for (int pass = 0; pass < 3; ++pass) {
-    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
-    hist[threadIdx.x] = hist[threadIdx.x + PG_SEL_THREADS] = 0;
-    __syncthreads();
+    for (int c = 0; c < CHUNKS; ++c) x[c] = pg_rows(P, P.weights + b * P.wb + head * P.wh, n, c);
+    uint32_t lowest = 0, known = 0;   // bits of the lowest kept order found so far
+    int need = P.budget;
+#pragma unroll 1
+    for (int pass = 0; pass < 3; ++pass) {
+      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
+      hist[threadIdx.x] = hist[threadIdx.x + PG_SEL_THREADS] = 0;
+      __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (x.o[i] && (x.o[i] & known) == lowest) atomicAdd(&hist[(x.o[i] >> shift) & (bins - 1)], 1);
-    lowest |= (uint32_t)pg_pick(hist, bins, need) << shift;
-    known |= (uint32_t)(bins - 1) << shift;
-    __syncthreads();
+      for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (x[c].o[i] && (x[c].o[i] & known) == lowest) atomicAdd(&hist[(x[c].o[i] >> shift) & (bins - 1)], 1);
+      lowest |= (uint32_t)pg_pick(hist, bins, need) << shift;
+      known |= (uint32_t)(bins - 1) << shift;
+      __syncthreads();
+    }
+    int base = 0, ties = 0;
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c)
+      if (c * PG_CHUNK < n) pg_emit(P, g, b, head, x[c], lowest, need, base, ties);
   }
-  pg_emit(P, g, b, head, x, lowest, need, 0, 0);
 }
 
 // Longer prompts: four launches over all chunks, one of them over the rows in question only.  1: the chunks' rows by the first
@@ -864,7 +877,8 @@ __global__ __launch_bounds__(PG_SEL_THREADS) void paged_list_kernel(PagedFillPar
   if (chunk * PG_CHUNK >= n) return;
   if (n <= P.budget) return pg_whole(P, b, head, chunk * PG_CHUNK, min(n, (chunk + 1) * PG_CHUNK));
   const PagedRows x = pg_rows(P, P.weights + b * P.wb + head * P.wh, n, chunk);
-  const int2 limit = P.limit[g], at = P.counts[(size_t)g * P.chunks + chunk];
+  const int2 limit = P.limit[g];
+  int2 at = P.counts[(size_t)g * P.chunks + chunk];
   pg_emit(P, g, b, head, x, (uint32_t)limit.x, limit.y, at.x, at.y);
 }
 
@@ -1011,7 +1025,7 @@ extern "C" int ri_paged_append(const ri_paged_t* cache, const void* key, const v
 
 // 16-byte aligned parts of the workspace of a fill: kept, hist, coarse, tied, counts, limit
 static size_t paged_fill_carve(PagedFillParams* P, size_t groups, int T, int budget, char* at) {
-  const size_t chunks = T > PG_CHUNK ? ((size_t)T + PG_CHUNK - 1) / PG_CHUNK : 0;
+  const size_t chunks = T > PG_CHUNK * PG_SEL_CHUNKS ? ((size_t)T + PG_CHUNK - 1) / PG_CHUNK : 0;
   size_t used = 0;
   const auto part = [&](size_t bytes) {
     char* const p = at + used;
@@ -1077,9 +1091,13 @@ extern "C" int ri_paged_fill(const ri_paged_t* cache, const void* key, const voi
   hipStream_t s = (hipStream_t)stream;
   const dim3 each(cache->heads, B), chunks(P.chunks, cache->heads, B);
   if (T <= budget) {
-    if (scores || positions) paged_select_kernel<true><<<each, PG_SEL_THREADS, 0, s>>>(P);
+    if (scores || positions) paged_select_kernel<0><<<each, PG_SEL_THREADS, 0, s>>>(P);
+  } else if (T <= PG_CHUNK) {
+    paged_select_kernel<1><<<each, PG_SEL_THREADS, 0, s>>>(P);
+  } else if (T <= 2 * PG_CHUNK) {
+    paged_select_kernel<2><<<each, PG_SEL_THREADS, 0, s>>>(P);
   } else if (P.chunks == 0) {
-    paged_select_kernel<false><<<each, PG_SEL_THREADS, 0, s>>>(P);
+    paged_select_kernel<PG_SEL_CHUNKS><<<each, PG_SEL_THREADS, 0, s>>>(P);
   } else {
     paged_digit_kernel<<<chunks, PG_SEL_THREADS, 0, s>>>(P);
     paged_tied_kernel<<<chunks, PG_SEL_THREADS, 0, s>>>(P);

@@ -268,6 +268,10 @@ def test_append_without_scores_and_with_odd_ones(dev):
     (BF, 2, 8200, 1, 64, 32, 8100, None, 0, 4100, "zero"),
     (BF, 1, 12289, 2, 64, 32, 5000, [12288], 0, 0, "few"),
     (HF, 1, 16384, 1, 64, 128, 4097, None, 17, 0, "odd"),
+    (HF, 4, 17001, 2, 64, 64, 700, [17001, 4096, 16385, 100], 4, 64, "any"),
+    (BF, 2, 20500, 1, 64, 32, 20400, [20500, 20401], 0, 4100, "zero"),
+    (BF, 1, 24577, 1, 64, 32, 5000, [24576], 0, 0, "few"),
+    (HF, 1, 16400, 1, 64, 128, 4097, None, 17, 0, "odd"),
 ])
 def test_fill(dev, dt, B, T, heads, dim, page, budget, lens, sinks, recent, weights):
     gen = torch.Generator().manual_seed(T + page)

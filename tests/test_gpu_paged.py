@@ -272,6 +272,8 @@ def test_append_without_scores_and_with_odd_ones(dev):
     (BF, 2, 20500, 1, 64, 32, 20400, [20500, 20401], 0, 4100, "zero"),
     (BF, 1, 24577, 1, 64, 32, 5000, [24576], 0, 0, "few"),
     (HF, 1, 16400, 1, 64, 128, 4097, None, 17, 0, "odd"),
+    (BF, 26, 16385, 4, 64, 8, 21, [16385 - 631 * b for b in range(26)], 3, 2, "any"),    # more chunks than run at a time
+    (BF, 26, 16385, 4, 64, 8, 21, None, 0, 0, "few"),
 ])
 def test_fill(dev, dt, B, T, heads, dim, page, budget, lens, sinks, recent, weights):
     gen = torch.Generator().manual_seed(T + page)

@@ -276,21 +276,26 @@ __global__ __launch_bounds__(64 * PG_WAVES, UNI && GP < 16 ? 4 : 2) void paged_a
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) *reinterpret_cast<uint4*>(vt + (lane / LPR + RPI * i) * VS + (lane % LPR) * 8) = v[i];
+    pg_heads<NH> sv;
+#pragma unroll
+    for (int i = 0; i < NH; ++i) {
+      const int r = GP == 16 ? i : rsel + i;
+      const float x = r == 0 ? s4[0] : r == 1 ? s4[1] : r == 2 ? s4[2] : s4[3];
+      sv.x[i] = valid ? x * P.scale2 : -INFINITY;
+    }
+    // A lane's heads are neighbours, and a chunk's scores one piece of memory.  (In front of the next loads: whoever waits for these
+    // waits for what was stored before, too.)
+    if (P.logits && rk < w1) *reinterpret_cast<pg_heads<NH>*>(P.logits + ((size_t)g * P.max_len + rk) * GP + head_of(0)) = sv;
     if (c + PG_WAVES < c1) {
       pages(c + PG_WAVES);
       load_keys(c + PG_WAVES);
       load_values(c + PG_WAVES);
     }
     float al[NH];
-    pg_heads<NH> sv;
     bool rescale = false;
 #pragma unroll
     for (int i = 0; i < NH; ++i) {
-      const int r = GP == 16 ? i : rsel + i;
-      const float x = r == 0 ? s4[0] : r == 1 ? s4[1] : r == 2 ? s4[2] : s4[3];
-      const float s = valid ? x * P.scale2 : -INFINITY;
-      sv.x[i] = s;
-      const float mn = fmaxf(m[i], pg_row_max(s));
+      const float s = sv.x[i], mn = fmaxf(m[i], pg_row_max(s));
       const bool none = mn == -INFINITY;   // relative to -inf they would weigh NaN
       al[i] = none ? 1.f : pg_exp2(m[i] - mn);
       const float p = pg_exp2(s - (none ? 0.f : mn));
@@ -299,8 +304,6 @@ __global__ __launch_bounds__(64 * PG_WAVES, UNI && GP < 16 ? 4 : 2) void paged_a
       m[i] = mn;
       pb[head_of(i) * 16 + n] = ri_f32_to_e16<HALF>(p);
     }
-    // (a lane's heads are neighbours, and a chunk's scores one piece of memory)
-    if (P.logits && rk < w1) *reinterpret_cast<pg_heads<NH>*>(P.logits + ((size_t)g * P.max_len + rk) * GP + head_of(0)) = sv;
     const bool any = __builtin_amdgcn_ballot_w64(rescale) != 0;
     if (any && n == 0) {
 #pragma unroll

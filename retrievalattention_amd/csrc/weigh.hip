@@ -2,7 +2,7 @@
 //
 // w[j] = sum over the query heads of a key-value head and over the last W tokens i of a prompt of exp(s_ij - lse_i), with
 // s_ij = scale q_i.k_j for keys j up to the query's own token and lse_i = log sum_j exp(s_ij): column sums of the attention
-// matrix, which is never stored.  The sums need every row's lse first, so the product is made twice: once for the lse of each
+// matrix, which is never stored.  The sums need every row's lse first, so the product is made twice: once for that of each
 // (query, head), called a column here, and once for the sums.  A tile of it is 32 keys by 32 columns (MFMA 32x32x16), whose lane
 // l holds one column of the product, l % 32, and of its rows 8 (i / 4) + 4 (l / 32) + i % 4 as accumulator i: with the columns as
 // columns the sums over keys stay in the lane until all tiles are done, with the keys as columns those over columns do.
@@ -31,18 +31,21 @@ struct WeighParams {
   const int32_t* lens;    // [B] or null: T each
   float* out;             // [B, heads, T]
   float* stats;           // [B * heads, S, cols_pad, 2] maximum (units of ln 2) and sum of the splits
-  float* lse;             // [B * heads, cols_pad], units of ln 2; +inf: the column has no keys
+  float2* norms;          // [B * heads, cols_pad]: a column's reference (units of ln 2) and the inverse of its sum
   float* part;            // [B * heads, supers, T] their sums
   int heads, gs, W, T, cols, cols_pad;
   int S;                  // splits of the keys in the first pass
   int rows;               // keys of a split of the pass
   int per, supers;        // blocks of columns to a workgroup of the second pass, workgroups to all
-  int joined;             // whether lse is filled before the second kernel
+  int joined;             // whether norms is filled before the second pass
   float scale2;           // scale / ln 2
 };
 
-// The lse of a column from its splits, of which this thread takes `part`, part + of, ...; `of` neighbouring lanes together.
-__device__ __forceinline__ float weigh_join(const WeighParams& P, int g, int col, int part, int of) {
+// A column's reference M and the inverse of its sum relative to M, of which a weight is exp(s - M) / sum, from its splits: this
+// thread takes `part`, part + of, ...; `of` neighbouring lanes together.  (Not the log-sum-exp alone: rounded to 32 bits it shifts all
+// weights of the column by up to half a unit of its size, 7e-7 of them, which is most of the error of a few queries' weights.)
+// A column without keys: inf and 0, so that a score less inf weighs 0.
+__device__ __forceinline__ float2 weigh_join(const WeighParams& P, int g, int col, int part, int of) {
   const float* const at = P.stats + ((size_t)g * P.S * P.cols_pad + col) * 2;
   float M = -INFINITY, L = 0.f;
 #pragma unroll 4
@@ -57,7 +60,7 @@ __device__ __forceinline__ float weigh_join(const WeighParams& P, int g, int col
     L = L * __builtin_amdgcn_exp2f(M - ref) + l * __builtin_amdgcn_exp2f(m - ref);
     M = mn;
   }
-  return L != 0.f ? M + __log2f(L) : INFINITY;
+  return L != 0.f ? make_float2(M, 1.f / L) : make_float2(INFINITY, 0.f);
 }
 
 __device__ __forceinline__ int weigh_len(const WeighParams& P, int b) { return P.lens ? min(max(P.lens[b], 0), P.T) : P.T; }
@@ -101,7 +104,7 @@ __device__ __forceinline__ int weigh_last_key(const WeighParams& P, int n, int s
 
 // One pass over the keys [j0, j1) of a split of group blockIdx.x, of which the columns [32 wave, 32 wave + 32) of
 // a block of 32 WAVES see some.
-// SUM false: the lse, of a block's columns as columns of the product;
+// SUM false: references and sums, of a block's columns as columns of the product;
 // m and l of a lane: its reference and the sum of exponentials relative to it, over its own keys.  The reference is the maximum of
 // the first tile that the column sees, and moves only where a tile's sum passes 2^100: until then neither the sums nor their
 // precision suffer, and a score costs a product with its offset, an exponential and an addition.
@@ -109,9 +112,11 @@ __device__ __forceinline__ int weigh_last_key(const WeighParams& P, int n, int s
 // up in the lane; the waves leave theirs in LDS, where one of them adds up a tile's behind the barrier that follows.
 template <int D, bool HALF, bool SUM, int WAVES, int OCC>
 __global__ __launch_bounds__(64 * WAVES, OCC) void weigh_kernel(WeighParams P) {
-  constexpr int BLOCK = 32 * WAVES, LOADS = WG_TILE * D * 2 / (1024 * WAVES), KK = D / 16, EX = 16 / KK, RING = 4;   // EX: exponentials to a product; RING: operands read ahead
+  constexpr int BLOCK = 32 * WAVES, LOADS = WG_TILE * D * 2 / (1024 * WAVES), KK = D / 16, EX = 16 / KK,   // EX: exponentials to a product
+                RING = SUM && WAVES == 4 ? 2 : 4;   // operands read ahead (with 4 and the inverse sums 5 registers of the second pass spill: 334 us for 328)
+  static_assert(KK % RING == 0, "a sub-tile's first operand is the ring's first");
   __shared__ __attribute__((aligned(16))) uint16_t sh[WG_BUFFERS][WG_TILE * D];
-  __shared__ __attribute__((aligned(16))) float sh_lse[SUM ? BLOCK : 4];
+  __shared__ __attribute__((aligned(16))) float sh_ref[SUM ? BLOCK : 4], sh_inv[SUM ? BLOCK : 4];
   __shared__ float sh_part[SUM ? WG_BUFFERS : 1][SUM ? WAVES : 1][WG_TILE];
   extern __shared__ float sh_sum[];   // [rows], with several blocks
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -151,15 +156,17 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void weigh_kernel(WeighParams P) {
     const int j1 = min(jn, first + min(block * BLOCK + BLOCK - 1, P.cols - 1) / P.gs + 1);   // (the last key of the block)
     if (j0 >= j1) continue;
     const int tiles = (j1 - j0 + WG_TILE - 1) / WG_TILE, subs = (j1 - j0 + 31) / 32;
-    if (SUM) {   // the block's lse, joined from its splits where nobody has done so before
+    if (SUM) {   // the block's references and sums, joined from their splits where nobody has done so before
       if ((int)threadIdx.x < BLOCK) {
         const int col = block * BLOCK + threadIdx.x;
-        sh_lse[SUM ? threadIdx.x : 0] = P.joined ? P.lse[(size_t)g * P.cols_pad + col] : weigh_join(P, g, col, 0, 1);
+        const float2 x = P.joined ? P.norms[(size_t)g * P.cols_pad + col] : weigh_join(P, g, col, 0, 1);
+        sh_ref[SUM ? threadIdx.x : 0] = x.x;
+        sh_inv[SUM ? threadIdx.x : 0] = x.y;
       }
       __syncthreads();
     }
     uint4 q[KK];
-    f32x16_t off;               // SUM: minus the lse of the rows
+    f32x16_t off, inv;          // SUM: of the rows minus the reference, and the inverse sum
     const int col = min(colw + (lane & 31), P.cols - 1), qi = col / P.gs;
     const int low = first + min(colw, P.cols - 1) / P.gs, mine = first + qi;   // last keys of the tile's first and the lane's column
     {
@@ -169,8 +176,10 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void weigh_kernel(WeighParams P) {
       if (SUM) {
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          const float4 o = *reinterpret_cast<const float4*>(&sh_lse[wave * 32 + 8 * x + 4 * (lane >> 5)]);
+          const float4 o = *reinterpret_cast<const float4*>(&sh_ref[wave * 32 + 8 * x + 4 * (lane >> 5)]);
+          const float4 f = *reinterpret_cast<const float4*>(&sh_inv[wave * 32 + 8 * x + 4 * (lane >> 5)]);
           off[4 * x] = -o.x; off[4 * x + 1] = -o.y; off[4 * x + 2] = -o.z; off[4 * x + 3] = -o.w;
+          inv[4 * x] = f.x; inv[4 * x + 1] = f.y; inv[4 * x + 2] = f.z; inv[4 * x + 3] = f.w;
         }
       }
       // waited for here, so that no wait for them stands between those for the tiles
@@ -263,9 +272,12 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void weigh_kernel(WeighParams P) {
           const float scale2 = u ? mask(j0 + 32 * u - 32) : 1.f;
           f32x16_t p = zero;
           float sum = 0.f, x = 0.f, e[EX];
-          const auto add = [&]() {   // (two sums, so that an addition does not wait for the one before)
+          const auto add = [&](int kk) {   // the products' kk; two sums, so that an addition does not wait for the one before
 #pragma unroll
-            for (int i = 0; i < EX; i += 2) { sum += e[i]; x += e[i + 1]; }
+            for (int i = 0; i < EX; i += 2) {
+              sum = SUM ? fmaf(e[i], inv[EX * kk + i], sum) : sum + e[i];
+              x = SUM ? fmaf(e[i + 1], inv[EX * kk + i + 1], x) : x + e[i + 1];
+            }
           };
 #pragma unroll
           for (int kk = 0; kk < KK; ++kk) {
@@ -273,7 +285,7 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void weigh_kernel(WeighParams P) {
             p = SUM ? weigh_mfma<HALF>(q[kk], from, p) : weigh_mfma<HALF>(from, q[kk], p);
             from = kk + RING < KK ? operand(buf, sub, kk + RING)
                                   : sub ? operand((buf + 1) % WG_BUFFERS, 0, kk + RING - KK) : operand(buf, 1, kk + RING - KK);
-            if (kk) add();
+            if (kk) add(kk - 1);
 #pragma unroll
             for (int i = 0; i < EX; ++i)
               e[i] = __builtin_amdgcn_exp2f(fmaf(s[EX * kk + i], scale2, SUM ? off[EX * kk + i] : -m));
@@ -282,7 +294,7 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void weigh_kernel(WeighParams P) {
             for (int i = 0; i < EX; i += 2) asm volatile("" : "+v"(e[i]), "+v"(e[i + 1]), "+v"(q[(kk + 1) % KK].x));
             __builtin_amdgcn_sched_barrier(0);
           }
-          add();
+          add(KK - 1);
           if (u) finish(sum + x, scale2, sub ? buf : (buf + WG_BUFFERS - 1) % WG_BUFFERS, sub ^ 1);
           s = p;
         }
@@ -292,7 +304,10 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void weigh_kernel(WeighParams P) {
       const float scale2 = mask(j0 + 32 * subs - 32);
       float sum = 0.f;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) sum += __builtin_amdgcn_exp2f(fmaf(s[i], scale2, SUM ? off[i] : -m));
+      for (int i = 0; i < 16; ++i) {
+        const float e = __builtin_amdgcn_exp2f(fmaf(s[i], scale2, SUM ? off[i] : -m));
+        sum = SUM ? fmaf(e, inv[i], sum) : sum + e;
+      }
       finish(sum, scale2, (tiles - 1) % WG_BUFFERS, (subs - 1) & 1);
     }
     if (SUM) {
@@ -323,8 +338,8 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void weigh_kernel(WeighParams P) {
 // Grid (cols_pad / 32, B * heads), 256 threads: eight threads join the splits of a column.
 __global__ __launch_bounds__(256) void weigh_join_kernel(WeighParams P) {
   const int g = blockIdx.y, col = blockIdx.x * 32 + (threadIdx.x >> 3);
-  const float lse = weigh_join(P, g, col, threadIdx.x & 7, 8);
-  if ((threadIdx.x & 7) == 0) P.lse[(size_t)g * P.cols_pad + col] = lse;
+  const float2 x = weigh_join(P, g, col, threadIdx.x & 7, 8);
+  if ((threadIdx.x & 7) == 0) P.norms[(size_t)g * P.cols_pad + col] = x;
 }
 
 // Grid (ceil(T / 256), B * heads): a thread adds the parts of a key, of those that have columns that see it.
@@ -380,7 +395,7 @@ extern "C" size_t ri_attention_weights_workspace_bytes(int B, int heads, int gs,
       (int64_t)W * gs > (int64_t)65535 * WG_SUM_COLS)   // (dimensions of grids)
     return 0;
   const WeighPlan p = weigh_plan((int64_t)B * heads, W * gs, T);
-  return (size_t)B * heads * ((size_t)p.cols_pad * (2 * (size_t)p.S + (p.joined ? 1 : 0)) + (p.supers > 1 ? (size_t)p.supers * T : 0)) * sizeof(float);
+  return (size_t)B * heads * ((size_t)p.cols_pad * 2 * ((size_t)p.S + (p.joined ? 1 : 0)) + (p.supers > 1 ? (size_t)p.supers * T : 0)) * sizeof(float);
 }
 
 template <int D, bool HALF>
@@ -411,10 +426,10 @@ static int attention_weights_impl(const void* q, const void* key, const int32_t*
   const int cols = W * gs, groups = B * heads;
   const WeighPlan p = weigh_plan(groups, cols, T);
   float* const stats = (float*)workspace;
-  float* const lse = stats + (size_t)groups * p.cols_pad * 2 * p.S;
+  float* const norms = stats + (size_t)groups * p.cols_pad * 2 * p.S;
   const WeighParams P = {(const uint16_t*)q, (const uint16_t*)key, q_batch_stride, q_token_stride, q_head_stride, key_batch_stride,
-                         key_token_stride, key_head_stride, seqlens, out, stats, lse,
-                         lse + (p.joined ? (size_t)groups * p.cols_pad : 0), heads, gs, W, T, cols, p.cols_pad, p.S, p.rows, p.per,
+                         key_token_stride, key_head_stride, seqlens, out, stats, (float2*)norms,
+                         norms + (p.joined ? 2 * (size_t)groups * p.cols_pad : 0), heads, gs, W, T, cols, p.cols_pad, p.S, p.rows, p.per,
                          p.supers, p.joined, scale * WG_LOG2E};
   hipStream_t s = (hipStream_t)stream;
   if (dim == 64) half ? launch_weigh<64, true>(P, p, groups, s) : launch_weigh<64, false>(P, p, groups, s);

@@ -381,6 +381,17 @@ def test_prompt_weights_scales(dev, scale):
     assert bool(((got.cpu().double() - want).abs() <= rel * want + 1e-30).all())
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("T", [3, 7, 31])
+def test_prompt_weights_of_equal_keys(dev, T, dim):
+    """One query, T equal keys: each exponential is that of 0 whatever the score, sums are whole numbers, and the weight 1 / T
+    carries one rounding of the inverse (another's room for the division), however large the score is."""
+    gen = torch.Generator().manual_seed(T)
+    q, key = _randn(gen, 8, 1, 16, dim).to(BF), (3 * _randn(gen, 8, 1, 16, dim)).to(BF).expand(8, T, 16, dim)
+    got = kernels.attention_weights(q.to(dev), key.to(dev)).cpu().double()
+    assert bool(((got * T - 1).abs() <= 2 * F).all())
+
+
 def test_prompt_weights_far_apart(dev):
     """Scores that rise along the prompt by more than an exponential of fp32 can tell, and fall."""
     gen = torch.Generator().manual_seed(10)

@@ -98,6 +98,8 @@ class paged_cache:
         """One sequence's prompt in one layer: query [1, T, heads, dim] (only read with a budget), key and value [1, T, kv heads,
         dim].  Returns key and value as they came, for the prompt's own attention."""
         T, b = key_states.shape[1], batch_idx
+        if not 0 <= b < self.batch_size or T < 1 or key_states.shape[0] != 1:
+            raise ValueError(f"paged_cache: expected a prompt [1, 1 token or more, ..] and a place below {self.batch_size}")
         if layer_idx == 0:
             if self.budget is None and T > self.rows:
                 raise ValueError(f"paged_cache: a prompt of {T} tokens, built for {self.rows}")

@@ -60,6 +60,10 @@ __device__ __forceinline__ f32x4_t pg_mfma16(pg_s4 a, pg_s4 b, f32x4_t c) {
               : __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a, b, c, 0, 0, 0);
 }
 
+// What a part's sums weigh relative to the maximum M of all.  A part without rows and one whose scores are all NaN have no maximum: its
+// own sum, 0 or NaN, stands in, so that a NaN arrives.
+__device__ __forceinline__ float pg_weigh_part(float m, float l, float M) { return m == -INFINITY ? l : pg_exp2(m - M); }
+
 // maximum / sum over the 16 lanes of a row, in every lane
 __device__ __forceinline__ float pg_row_max(float x) { return ri_xor_max<1>(ri_xor_max<2>(ri_xor_max<4>(ri_xor_max<8>(x)))); }
 __device__ __forceinline__ float pg_row_sum(float x) { return ri_xor_sum<1>(ri_xor_sum<2>(ri_xor_sum<4>(ri_xor_sum<8>(x)))); }
@@ -359,7 +363,7 @@ __global__ __launch_bounds__(64 * PG_WAVES, UNI && GP < 16 ? 4 : 2) void paged_a
     for (int w = 0; w < PG_WAVES; ++w) M = fmaxf(M, sh_m[w][j]);
 #pragma unroll
     for (int w = 0; w < PG_WAVES; ++w) {
-      const float f = sh_m[w][j] == -INFINITY ? 0.f : pg_exp2(sh_m[w][j] - M);
+      const float f = pg_weigh_part(sh_m[w][j], sh_l[w][j], M);
       L += sh_l[w][j] * f;
       A += ((const float*)sh_tile[w])[j * D + d] * f;
     }
@@ -413,13 +417,12 @@ __global__ __launch_bounds__(PG_JOIN_THREADS) void paged_join_kernel(PagedAttend
     float M = -INFINITY, L = 0.f;
     for (int s = lane; s < parts; s += 64) M = fmaxf(M, ml[(size_t)s * GP + j].x);
     M = ri_wave_max(M);
-    if (M != -INFINITY)
-      for (int s = lane; s < parts; s += 64) {
-        const float2 x = ml[(size_t)s * GP + j];
-        const float f = pg_exp2(x.x - M);
-        if (joins) sh_f[s] = f;
-        L += x.y * f;
-      }
+    for (int s = lane; s < parts; s += 64) {
+      const float2 x = ml[(size_t)s * GP + j];
+      const float f = pg_weigh_part(x.x, x.y, M);
+      if (joins) sh_f[s] = f;
+      L += x.y * f;
+    }
     L = ri_wave_sum(L);
     if (lane == 0) {
       sh_M[j] = M;
@@ -432,21 +435,19 @@ __global__ __launch_bounds__(PG_JOIN_THREADS) void paged_join_kernel(PagedAttend
     __syncthreads();
     const float M = sh_M[j], L = sh_L[j];
     float A[DL] = {};
-    if (M != -INFINITY) {
-      const float* const acc = P.part_acc + (part0 * GP + j) * D + DL * lane;
-      for (int s = wave; s < parts; s += U * NW) {
-        float x[U][DL];
+    const float* const acc = P.part_acc + (part0 * GP + j) * D + DL * lane;
+    for (int s = wave; s < parts; s += U * NW) {
+      float x[U][DL];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+      for (int u = 0; u < U; ++u)
 #pragma unroll
-          for (int d = 0; d < DL; ++d) x[u][d] = acc[(size_t)min(s + u * NW, parts - 1) * GP * D + d];
+        for (int d = 0; d < DL; ++d) x[u][d] = acc[(size_t)min(s + u * NW, parts - 1) * GP * D + d];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-          if (s + u * NW < parts) {
+      for (int u = 0; u < U; ++u)
+        if (s + u * NW < parts) {
 #pragma unroll
-            for (int d = 0; d < DL; ++d) A[d] += x[u][d] * sh_f[s + u * NW];
-          }
-      }
+          for (int d = 0; d < DL; ++d) A[d] += x[u][d] * sh_f[s + u * NW];
+        }
     }
 #pragma unroll
     for (int d = 0; d < DL; ++d) sh_a[wave][DL * lane + d] = A[d];
@@ -1114,6 +1115,7 @@ extern "C" int ri_paged_fill(const ri_paged_t* cache, const void* key, const voi
     return RI_ERR_ARG;
   const int room = T < budget ? T : budget;
   if ((T > budget || scores) && !weights) return RI_ERR_ARG;
+  if (scores && scores == weights) return RI_ERR_ARG;   // (written while others still read)
   if (weights && (weight_head_stride < T || weight_batch_stride < 0)) return RI_ERR_ARG;
   if (scores && (score_head_stride < room || score_batch_stride < 0)) return RI_ERR_ARG;
   if (positions && (position_head_stride < room || position_batch_stride < 0)) return RI_ERR_ARG;

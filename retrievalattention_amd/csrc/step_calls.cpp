@@ -516,7 +516,8 @@ PyObject* paged_fill(PyObject*, PyObject* const* args, Py_ssize_t n) {
       (held && lens && held->data_ptr() == lens->data_ptr()) ||
       !paged_values(args[7], at::kFloat, B, cache.heads, T, device, false, &weights, ws) ||
       !paged_values(args[8], at::kFloat, B, cache.heads, rows, device, true, &scores, ss) ||
-      !paged_values(args[9], at::kInt, B, cache.heads, rows, device, true, &positions, ps) || (!weights && (T > budget || scores)))
+      !paged_values(args[9], at::kInt, B, cache.heads, rows, device, true, &positions, ps) || (!weights && (T > budget || scores)) ||
+      (scores && scores->data_ptr() == weights->data_ptr()))
     Py_RETURN_NONE;
   const size_t bytes = ri_paged_fill_workspace_bytes((int)B, cache.heads, (int)T, (int)budget);
   void* const work = bytes ? paged_scratch(args[13], bytes, device) : nullptr;

@@ -946,7 +946,7 @@ def paged_append(key, value, k_pages, v_pages, block_table, cache_seqlens, new_s
     the table holds) takes them as its next row; in a full one, given `scores` [B, heads, rows] fp32, `positions` [B, heads, rows]
     int32 and `token_positions` [B] int32 (the token's place in its sequence), they take the place of the row with the lowest score
     in each head, the first `sinks` and the last `recent` tokens of the sequence (the new one is the last) excepted; equal scores:
-    the lowest row; a NaN counts as the highest.  The row's score becomes 0, its position the token's.  A full sequence without
+    the lowest row; a NaN counts as the highest; where positions except every row: row 0.  The row's score becomes 0, its position the token's.  A full sequence without
     scores is left as it is.  The page that takes the row must be no other sequence's.
     new_seqlens [B] int32, another tensor than cache_seqlens: the rows in use afterwards."""
     status = step_calls().paged_append(key, value, k_pages, v_pages, block_table, cache_seqlens, new_seqlens, scores, positions,
@@ -987,8 +987,9 @@ def paged_fill(key, value, k_pages, v_pages, block_table, new_seqlens=None, seql
     """Writes prompts, key and value [B, T, heads, dim], into the pages from row 0 on; seqlens [B] int32: their lengths (default
     T).  Of a prompt of more than `budget` tokens (default: the rows that the table holds) each head keeps `budget`: the first
     `sinks`, the last `recent` and of the others those with the highest weights [B, heads, T] fp32 (attention_weights), at equal
-    weights the first ones, in their order.  new_seqlens [B] int32: the rows written.  scores, positions [B, heads, rows]: take the
-    kept weights and the tokens' places.  A sequence's pages must be no other's."""
+    weights the first ones, in their order.  new_seqlens [B] int32: the rows written.  scores (other
+    memory than weights), positions [B, heads, rows]: take the kept weights and the tokens' places.  A sequence's pages must be no
+    other's."""
     status = step_calls().paged_fill(key, value, k_pages, v_pages, block_table, new_seqlens, seqlens, weights, scores, positions,
                                      budget, sinks, recent, _held(key, "paged_fill", scratch))
     if status is not None:
@@ -1015,6 +1016,8 @@ def paged_fill(key, value, k_pages, v_pages, block_table, new_seqlens=None, seql
     wb, wh = _per_row(weights, torch.float32, B, cache.heads, T, device, "weights", writes=False)
     sb, sh = _per_row(scores, torch.float32, B, cache.heads, min(T, budget), device, "scores")
     pb, ph = _per_row(positions, torch.int32, B, cache.heads, min(T, budget), device, "positions")
+    if scores is not None and scores.data_ptr() == weights.data_ptr():
+        raise ValueError("scores: expected other memory than weights")
     with _on(device):
         nbytes = lib().ri_paged_fill_workspace_bytes(B, cache.heads, T, budget)
         ws = _workspace(nbytes, device, "paged_fill", scratch) if nbytes else None

@@ -111,6 +111,35 @@ def test_attention(dev, dt, B, heads, gs, dim, page, lens, starts, scored):
     assert torch.equal(again, out)   # no order of arrival in the result
 
 
+@pytest.mark.parametrize("lens", [[5, 16], [200, 331], [3, 5000]])
+@pytest.mark.parametrize("what", ["query", "keys"])
+def test_attention_passes_nan_on(dev, lens, what):
+    """A NaN in what is attended is in the result, also where a part's scores are nothing else; other heads are as without it."""
+    gen = torch.Generator().manual_seed(lens[1])
+    B, heads, gs, dim = 2, 2, 3, 128
+    k, v, table = _pool(gen, BF, B, heads, dim, 16, lens[1])
+    q = (2 * _randn(gen, B, 1, heads * gs, dim)).to(BF)
+    on = lambda t: t.to(dev)  # noqa: E731
+    lens = torch.tensor(lens, dtype=torch.int32)
+    room = table.shape[1] * 16
+    scores, was = torch.zeros(B, heads, room, device=dev), torch.zeros(B, heads, room, device=dev)
+    want, want_lse = kernels.paged_attention(on(q), on(k), on(v), on(table), on(lens), scores=was, return_softmax_lse=True)
+    bad = torch.zeros(B, heads, gs, dtype=torch.bool)
+    if what == "query":
+        bad[0, 1, 2] = bad[1, 0, 0] = True
+        q[0, 0, gs + 2, 7], q[1, 0, 0, 127] = math.nan, math.nan
+    else:
+        bad[1, 1] = True
+        k[table[1].long(), 1] = math.nan
+    out, lse = kernels.paged_attention(on(q), on(k), on(v), on(table), on(lens), scores=scores, return_softmax_lse=True)
+    bad = bad.view(B, heads * gs)
+    assert bool(out.cpu()[:, 0][bad].isnan().all()) and torch.equal(out.cpu()[:, 0][~bad], want.cpu()[:, 0][~bad])
+    assert bool(lse.cpu()[bad].isnan().all()) and torch.equal(lse.cpu()[~bad], want_lse.cpu()[~bad])
+    attended = torch.arange(room)[None, None] < lens[:, None, None]
+    spoilt = bad.view(B, heads, gs).any(-1)[:, :, None] & attended
+    assert bool(scores.cpu()[spoilt].isnan().all()) and torch.equal(scores.cpu()[~spoilt], was.cpu()[~spoilt])
+
+
 def test_attention_max_len_scale_and_strides(dev):
     """Pages as [pages, rows, heads, dim], keys and values in one tensor, a table that is a part of a larger one, rows past max_len
     and pages that are not there left out, a scale of its own."""
@@ -379,6 +408,13 @@ def test_prompt_weights_scales(dev, scale):
     got = kernels.attention_weights(q.to(dev), key.to(dev), scale=scale)
     rel = 4 * (64 + 12) * F * (1 + size.abs()) + (64 + 300 / 32 + 150 / 32) * F
     assert bool(((got.cpu().double() - want).abs() <= rel * want + 1e-30).all())
+
+
+def test_fill_refuses_scores_in_place(dev):
+    x, table = torch.zeros(3, 1, 16, 64, dtype=BF, device=dev), torch.arange(2, dtype=torch.int32, device=dev)[None]
+    row, w = torch.zeros(1, 40, 1, 64, dtype=BF, device=dev), torch.rand(1, 1, 40, device=dev)
+    with pytest.raises(ValueError, match="other memory"):
+        kernels.paged_fill(row, row, x, x.clone(), table, weights=w, scores=w)
 
 
 @pytest.mark.parametrize("dim", [64, 128])

@@ -33,6 +33,15 @@ def _owned(cache):
     return [len(row) for row in cache._table]
 
 
+def test_refused_prompts_take_nothing():
+    c = _cache()
+    _prompt(c, 1, 5)
+    for b, T in ((-1, 5), (3, 5), (0, 0)):
+        with pytest.raises(ValueError, match="expected a prompt"):
+            _prompt(c, b, T)
+    assert _owned(c) == [0, 1, 0]
+
+
 def test_pages_follow_the_rows():
     c = _cache()
     _prompt(c, 0, 16)

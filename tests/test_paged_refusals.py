@@ -40,7 +40,7 @@ def _append(cache=None, **change):
 
 def _fill(cache=None, **change):
     a = dict(key=A, value=A, kb=25600, kt=256, kh=128, vb=25600, vt=256, vh=128, lens=A, weights=A, wb=200, wh=100, new=A + 64,
-             scores=A, sb=128, sh=64, positions=A, pb=128, ph=64, B=3, T=100, budget=64, sinks=4, recent=8, ws=A, bytes=1 << 20,
+             scores=2 * A, sb=128, sh=64, positions=A, pb=128, ph=64, B=3, T=100, budget=64, sinks=4, recent=8, ws=A, bytes=1 << 20,
              stream=None)
     a.update(change)
     return lib().ri_paged_fill(cache or _cache(), *a.values())
@@ -85,7 +85,8 @@ def test_append(bad):
 
 @pytest.mark.parametrize("bad", [dict(key=None), dict(value=A + 2), dict(kt=4), dict(vb=-8), dict(weights=None), dict(T=0), dict(B=0),
                                  dict(T=2 ** 24 + 1, wh=2 ** 25), dict(wh=99), dict(budget=0), dict(budget=65), dict(sinks=57),
-                                 dict(sinks=-1), dict(recent=-1), dict(sh=63), dict(ph=63), dict(ws=None), dict(pb=-1)], ids=str)
+                                 dict(sinks=-1), dict(recent=-1), dict(sh=63), dict(ph=63), dict(ws=None), dict(pb=-1),
+                                 dict(scores=A), dict(T=64, scores=A)], ids=str)
 def test_fill(bad):
     assert _fill(**bad) == ARG
 

@@ -342,24 +342,34 @@ __global__ __launch_bounds__(256) void weigh_join_kernel(WeighParams P) {
   if ((threadIdx.x & 7) == 0) P.norms[(size_t)g * P.cols_pad + col] = x;
 }
 
-// Grid (ceil(T / 256), B * heads): a thread adds the parts of a key, of those that have columns that see it.
+// Grid (ceil(T / KEYS), B * heads): 256 / KEYS threads add the parts of a key, of those that have columns that see it, every
+// so-many-th each.
+template <int KEYS>
 __global__ __launch_bounds__(256) void weigh_add_kernel(WeighParams P) {
-  const int g = blockIdx.y, j = blockIdx.x * 256 + threadIdx.x, n = weigh_len(P, g / P.heads);
-  if (j >= P.T) return;
+  constexpr int OF = 256 / KEYS;
+  __shared__ float sh[OF][KEYS];
+  const int g = blockIdx.y, at = threadIdx.x % KEYS, mine = threadIdx.x / KEYS, j = blockIdx.x * KEYS + at, n = weigh_len(P, g / P.heads);
   float x = 0.f;
   if (j < n) {
     const float* const from = P.part + (size_t)g * P.supers * P.T + j;
-    int s = max(j - (n - P.W), 0) * P.gs / (WG_SUM_COLS * P.per);
-    for (; s + 8 <= P.supers; s += 8) {
+    int s = max(j - (n - P.W), 0) * P.gs / (WG_SUM_COLS * P.per) + mine;
+    for (; s + 7 * OF < P.supers; s += 8 * OF) {
       float v[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = from[(size_t)(s + i) * P.T];
+      for (int i = 0; i < 8; ++i) v[i] = from[(size_t)(s + i * OF) * P.T];
 #pragma unroll
       for (int i = 0; i < 8; ++i) x += v[i];
     }
-    for (; s < P.supers; ++s) x += from[(size_t)s * P.T];
+    for (; s < P.supers; s += OF) x += from[(size_t)s * P.T];
   }
-  P.out[(size_t)g * P.T + j] = x;
+  if (OF > 1) {
+    sh[mine][at] = x;
+    __syncthreads();
+    if (mine) return;
+#pragma unroll
+    for (int i = 1; i < OF; ++i) x += sh[i][at];
+  }
+  if (j < P.T) P.out[(size_t)g * P.T + j] = x;
 }
 
 // ------------------------------------------------------------------------------------ host side
@@ -408,7 +418,9 @@ static void launch_weigh(WeighParams P, const WeighPlan& p, int groups, hipStrea
     weigh_kernel<D, HALF, true, WG_COLS / 32, 2><<<grid, 2 * WG_COLS, 0, s>>>(P);
   } else {
     weigh_kernel<D, HALF, true, WG_SUM_COLS / 32, 3><<<grid, 2 * WG_SUM_COLS, P.per > 1 ? P.rows * sizeof(float) : 0, s>>>(P);
-    if (P.supers > 1) weigh_add_kernel<<<dim3((P.T + 255) / 256, groups), 256, 0, s>>>(P);
+    // (256 parts of 65536 sums: eight threads to one 9.8 us, one 16)
+    if (P.supers >= 16) weigh_add_kernel<32><<<dim3((P.T + 31) / 32, groups), 256, 0, s>>>(P);
+    else if (P.supers > 1) weigh_add_kernel<256><<<dim3((P.T + 255) / 256, groups), 256, 0, s>>>(P);
   }
 }
 

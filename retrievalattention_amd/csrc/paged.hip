@@ -306,7 +306,7 @@ __global__ __launch_bounds__(64 * PG_WAVES, UNI && GP < 16 ? 4 : 2) void paged_a
       rescale |= al[i] != 1.f;
       l[i] = l[i] * al[i] + p;
       m[i] = mn;
-      pb[head_of(i) * 16 + n] = ri_f32_to_e16<HALF>(p);
+      pb[head_of(i) * 16 + n] = ri_f32_to_e16<HALF>(p);   // (half a step of a probability, for the matrix cores; sums are of p itself)
     }
     const bool any = __builtin_amdgcn_ballot_w64(rescale) != 0;
     if (any && n == 0) {

@@ -947,6 +947,11 @@ __global__ __launch_bounds__(256) void paged_copy_kernel(PagedFillParams P) {
 #define PG_MAX_ROWS (1 << 24)   // rows of a sequence
 static bool strides_ok(int64_t a, int64_t b, int64_t c = 0) { return a >= 0 && b >= 0 && c >= 0 && (a | b | c) % 8 == 0; }
 
+// two tables of n, one of which is written while others may still read the other
+static bool pg_meet(const int32_t* a, const int32_t* b, int n) {
+  return a && b && (uintptr_t)a < (uintptr_t)(b + n) && (uintptr_t)b < (uintptr_t)(a + n);
+}
+
 static int paged_view(const ri_paged_t* c, int B, PagedView* v) {
   if (!c || !c->k_pages || !c->v_pages || !c->block_table || ri_any_misaligned16(c->k_pages, c->v_pages)) return RI_ERR_ARG;
   if (c->pages <= 0 || c->heads <= 0 || c->table_pages <= 0 || B <= 0 || c->table_stride < 0) return RI_ERR_ARG;
@@ -1045,7 +1050,8 @@ extern "C" int ri_paged_append(const ri_paged_t* cache, const void* key, const v
                                const int32_t* token_positions, int B, int budget, int sinks, int recent, ri_stream_t stream) {
   PagedAppendParams P = {};
   if (const int rc = paged_view(cache, B, &P.c)) return rc;
-  if (!key || !value || !lens || lens == new_lens || ri_any_misaligned16(key, value)) return RI_ERR_ARG;
+  if (!key || !value || !lens || ri_any_misaligned16(key, value) || cache->k_pages == cache->v_pages) return RI_ERR_ARG;
+  if (pg_meet(lens, new_lens, B) || pg_meet(token_positions, new_lens, B)) return RI_ERR_ARG;
   if (!strides_ok(key_batch_stride, key_head_stride) || !strides_ok(value_batch_stride, value_head_stride)) return RI_ERR_ARG;
   if (budget <= 0 || budget > cache->table_pages * cache->page_rows || sinks < 0 || recent < 0 || (int64_t)sinks + recent >= budget)
     return RI_ERR_ARG;
@@ -1108,7 +1114,7 @@ extern "C" int ri_paged_fill(const ri_paged_t* cache, const void* key, const voi
                              int recent, void* workspace, size_t workspace_bytes, ri_stream_t stream) {
   PagedFillParams P = {};
   if (const int rc = paged_view(cache, B, &P.c)) return rc;
-  if (!key || !value || ri_any_misaligned16(key, value)) return RI_ERR_ARG;
+  if (!key || !value || ri_any_misaligned16(key, value) || cache->k_pages == cache->v_pages || pg_meet(seqlens, new_lens, B)) return RI_ERR_ARG;
   if (!strides_ok(key_batch_stride, key_token_stride, key_head_stride) || !strides_ok(value_batch_stride, value_token_stride, value_head_stride))
     return RI_ERR_ARG;
   if (T <= 0 || T > PG_MAX_ROWS || budget <= 0 || budget > cache->table_pages * cache->page_rows || sinks < 0 || recent < 0 || (int64_t)sinks + recent > budget)

@@ -379,6 +379,11 @@ bool paged_each(PyObject* o, int64_t B, int device, const at::Tensor** out, bool
   if (!paged_tensor(o, 1, at::kInt, device, out, optional)) return false;
   return !*out || ((*out)->size(0) == B && (B == 1 || (*out)->stride(0) == 1));
 }
+bool paged_meet(const at::Tensor* a, const at::Tensor* b, int64_t B) {
+  if (!a || !b) return false;
+  const auto x = (uintptr_t)a->data_ptr(), y = (uintptr_t)b->data_ptr();
+  return x < y + 4 * B && y < x + 4 * B;
+}
 // a value to each row, [B, heads, rows or more]; strides by sequence and head
 bool paged_values(PyObject* o, at::ScalarType dtype, int64_t B, int64_t heads, int64_t rows, int device, bool writes,
                   const at::Tensor** out, int64_t* strides) {
@@ -473,10 +478,10 @@ PyObject* paged_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const int64_t room = (int64_t)cache.table_pages * cache.page_rows;
   if (!paged_int(args[10], room, &budget) || !integers(args + 11, 1, &sinks) || !integers(args + 12, 1, &recent) || budget < 1 ||
       budget > room || sinks + recent >= budget || !paged_each(args[5], B, device, &lens, false) ||
-      !paged_each(args[6], B, device, &held) || (held && held->data_ptr() == lens->data_ptr()) ||
+      !paged_each(args[6], B, device, &held) || paged_meet(held, lens, B) || cache.k_pages == cache.v_pages ||
       !paged_values(args[7], at::kFloat, B, cache.heads, budget, device, true, &scores, ss) ||
       !paged_values(args[8], at::kInt, B, cache.heads, budget, device, true, &positions, ps) ||
-      !paged_each(args[9], B, device, &token) || (scores && !positions) || (positions && !token))
+      !paged_each(args[9], B, device, &token) || paged_meet(held, token, B) || (scores && !positions) || (positions && !token))
     Py_RETURN_NONE;
   void *kp = key->data_ptr(), *vp = value->data_ptr(), *np = lens->data_ptr(), *hp = address(held), *sp = address(scores),
        *pp = address(positions), *tp = address(token);
@@ -513,7 +518,7 @@ PyObject* paged_fill(PyObject*, PyObject* const* args, Py_ssize_t n) {
     Py_RETURN_NONE;
   const int64_t rows = T < budget ? T : budget;
   if (!paged_each(args[5], B, device, &held) || !paged_each(args[6], B, device, &lens) ||
-      (held && lens && held->data_ptr() == lens->data_ptr()) ||
+      paged_meet(held, lens, B) || cache.k_pages == cache.v_pages ||
       !paged_values(args[7], at::kFloat, B, cache.heads, T, device, false, &weights, ws) ||
       !paged_values(args[8], at::kFloat, B, cache.heads, rows, device, true, &scores, ss) ||
       !paged_values(args[9], at::kInt, B, cache.heads, rows, device, true, &positions, ps) || (!weights && (T > budget || scores)) ||

@@ -854,6 +854,12 @@ def _table32(t, shape, device, name):
     return t.stride(0)
 
 
+def _apart(new, other, name):
+    """Two int32 tables [B], the first of which is written while others may still read the second."""
+    if new is not None and other is not None and abs(new.data_ptr() - other.data_ptr()) < 4 * new.shape[0]:
+        raise ValueError(f"new_seqlens: expected another tensor than {name}, in memory of its own")
+
+
 def _per_row(t, dtype, B, heads, rows, device, name, writes=True):
     """Strides (sequence, head) of a tensor [B, heads, rows or more] with a value to each row; (0, 0) for None."""
     if t is None:
@@ -885,6 +891,8 @@ def _paged(k_pages, v_pages, block_table, B, writes=False):
     pages, heads, rows, dim = k_pages.shape
     if v_pages.shape != k_pages.shape:
         raise ValueError("k_pages and v_pages: expected the same shape")
+    if writes and k_pages.data_ptr() == v_pages.data_ptr():
+        raise ValueError("k_pages and v_pages: written, and they share memory")
     if dim not in PAGED_DIMS or rows < 1 or rows & (rows - 1) or pages < 1 or heads < 1:
         raise ValueError("k_pages: expected [pages, heads, a power of two, 64 or 128]")
     ts = _table32(block_table, (B, None), device, "block_table")
@@ -948,7 +956,7 @@ def paged_append(key, value, k_pages, v_pages, block_table, cache_seqlens, new_s
     in each head, the first `sinks` and the last `recent` tokens of the sequence (the new one is the last) excepted; equal scores:
     the lowest row; a NaN counts as the highest; where positions except every row: row 0.  The row's score becomes 0, its position the token's.  A full sequence without
     scores is left as it is.  The page that takes the row must be no other sequence's.
-    new_seqlens [B] int32, another tensor than cache_seqlens: the rows in use afterwards."""
+    new_seqlens [B] int32, other memory than cache_seqlens and token_positions: the rows in use afterwards."""
     status = step_calls().paged_append(key, value, k_pages, v_pages, block_table, cache_seqlens, new_seqlens, scores, positions,
                                        token_positions, budget, sinks, recent)
     if status is not None:
@@ -968,12 +976,12 @@ def paged_append(key, value, k_pages, v_pages, block_table, cache_seqlens, new_s
     _table32(cache_seqlens, (B,), device, "cache_seqlens")
     if new_seqlens is not None:
         _table32(new_seqlens, (B,), device, "new_seqlens")
-        if new_seqlens.data_ptr() == cache_seqlens.data_ptr():
-            raise ValueError("new_seqlens: expected another tensor than cache_seqlens")
+        _apart(new_seqlens, cache_seqlens, "cache_seqlens")
     if (scores is not None and positions is None) or (positions is not None and token_positions is None):
         raise ValueError("paged_append: scores go with positions, and those with token_positions")
     if token_positions is not None:
         _table32(token_positions, (B,), device, "token_positions")
+        _apart(new_seqlens, token_positions, "token_positions")
     sb, sh = _per_row(scores, torch.float32, B, cache.heads, budget, device, "scores")
     pb, ph = _per_row(positions, torch.int32, B, cache.heads, budget, device, "positions")
     with _on(device):
@@ -987,7 +995,7 @@ def paged_fill(key, value, k_pages, v_pages, block_table, new_seqlens=None, seql
     """Writes prompts, key and value [B, T, heads, dim], into the pages from row 0 on; seqlens [B] int32: their lengths (default
     T).  Of a prompt of more than `budget` tokens (default: the rows that the table holds) each head keeps `budget`: the first
     `sinks`, the last `recent` and of the others those with the highest weights [B, heads, T] fp32 (attention_weights), at equal
-    weights the first ones, in their order.  new_seqlens [B] int32: the rows written.  scores (other
+    weights the first ones, in their order.  new_seqlens [B] int32, other memory than seqlens: the rows written.  scores (other
     memory than weights), positions [B, heads, rows]: take the kept weights and the tokens' places.  A sequence's pages must be no
     other's."""
     status = step_calls().paged_fill(key, value, k_pages, v_pages, block_table, new_seqlens, seqlens, weights, scores, positions,
@@ -1011,8 +1019,7 @@ def paged_fill(key, value, k_pages, v_pages, block_table, new_seqlens=None, seql
     for t, nm in ((seqlens, "seqlens"), (new_seqlens, "new_seqlens")):
         if t is not None:
             _table32(t, (B,), device, nm)
-    if seqlens is not None and new_seqlens is not None and seqlens.data_ptr() == new_seqlens.data_ptr():
-        raise ValueError("new_seqlens: expected another tensor than seqlens")
+    _apart(new_seqlens, seqlens, "seqlens")
     wb, wh = _per_row(weights, torch.float32, B, cache.heads, T, device, "weights", writes=False)
     sb, sh = _per_row(scores, torch.float32, B, cache.heads, min(T, budget), device, "scores")
     pb, ph = _per_row(positions, torch.int32, B, cache.heads, min(T, budget), device, "positions")

@@ -410,11 +410,19 @@ def test_prompt_weights_scales(dev, scale):
     assert bool(((got.cpu().double() - want).abs() <= rel * want + 1e-30).all())
 
 
-def test_fill_refuses_scores_in_place(dev):
+def test_writers_refuse_shared_memory(dev):
+    """What a call writes while it still reads it elsewhere."""
     x, table = torch.zeros(3, 1, 16, 64, dtype=BF, device=dev), torch.arange(2, dtype=torch.int32, device=dev)[None]
-    row, w = torch.zeros(1, 40, 1, 64, dtype=BF, device=dev), torch.rand(1, 1, 40, device=dev)
-    with pytest.raises(ValueError, match="other memory"):
-        kernels.paged_fill(row, row, x, x.clone(), table, weights=w, scores=w)
+    row, w, lens = torch.zeros(1, 40, 1, 64, dtype=BF, device=dev), torch.rand(1, 1, 40, device=dev), torch.ones(1, dtype=torch.int32, device=dev)
+    v, one, places = x.clone(), row[:, :1], torch.zeros(1, 1, 32, dtype=torch.int32, device=dev)
+    for call in (lambda: kernels.paged_fill(row, row, x, v, table, weights=w, scores=w),
+                 lambda: kernels.paged_fill(row, row, x, x, table, weights=w),
+                 lambda: kernels.paged_fill(row, row, x, v, table, lens, seqlens=lens, weights=w),
+                 lambda: kernels.paged_append(one, one, x, x, table, lens),
+                 lambda: kernels.paged_append(one, one, x, v, table, lens, lens),
+                 lambda: kernels.paged_append(one, one, x, v, table, lens, table[0, :1], positions=places, token_positions=table[0, :1])):
+        with pytest.raises(ValueError, match="memory"):
+            call()
 
 
 @pytest.mark.parametrize("dim", [64, 128])

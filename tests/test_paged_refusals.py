@@ -13,7 +13,7 @@ A = 1 << 20   # an aligned address; nothing is read from it
 
 
 def _cache(**change):
-    s = dict(k_pages=A, v_pages=A, block_table=A, k_page_stride=4096, k_head_stride=2048, k_row_stride=128, v_page_stride=4096,
+    s = dict(k_pages=A, v_pages=2 * A, block_table=A, k_page_stride=4096, k_head_stride=2048, k_row_stride=128, v_page_stride=4096,
              v_head_stride=2048, v_row_stride=128, table_stride=4, pages=9, heads=2, page_rows=16, dim=128, table_pages=4, half=0)
     s.update(change)
     return ctypes.byref(Paged(**s))
@@ -75,8 +75,8 @@ def test_attention_workspace(scored):
         assert lib().ri_paged_attention_workspace_bytes(*bad, scored) == 0
 
 
-@pytest.mark.parametrize("bad", [dict(key=None), dict(value=A + 2), dict(kb=4), dict(vh=-8), dict(lens=None), dict(new=A), dict(B=0),
-                                 dict(budget=0), dict(budget=65), dict(sinks=-1), dict(recent=-1), dict(sinks=56),
+@pytest.mark.parametrize("bad", [dict(key=None), dict(value=A + 2), dict(kb=4), dict(vh=-8), dict(lens=None), dict(new=A), dict(new=A + 8),
+                                 dict(token=A + 72), dict(B=0), dict(budget=0), dict(budget=65), dict(sinks=-1), dict(recent=-1), dict(sinks=56),
                                  dict(sinks=2 ** 31 - 1, recent=2 ** 31 - 1), dict(positions=None), dict(token=None),
                                  dict(sh=63), dict(ph=63), dict(sb=-1)], ids=str)
 def test_append(bad):
@@ -86,9 +86,14 @@ def test_append(bad):
 @pytest.mark.parametrize("bad", [dict(key=None), dict(value=A + 2), dict(kt=4), dict(vb=-8), dict(weights=None), dict(T=0), dict(B=0),
                                  dict(T=2 ** 24 + 1, wh=2 ** 25), dict(wh=99), dict(budget=0), dict(budget=65), dict(sinks=57),
                                  dict(sinks=-1), dict(recent=-1), dict(sh=63), dict(ph=63), dict(ws=None), dict(pb=-1),
-                                 dict(scores=A), dict(T=64, scores=A)], ids=str)
+                                 dict(scores=A), dict(T=64, scores=A), dict(new=A),
+                                 dict(new=A - 8)], ids=str)
 def test_fill(bad):
     assert _fill(**bad) == ARG
+
+
+def test_writes_to_pages_of_both():
+    assert _append(_cache(v_pages=A)) == ARG and _fill(_cache(v_pages=A)) == ARG
 
 
 def test_fill_workspace():

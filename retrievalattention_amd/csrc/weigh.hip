@@ -156,6 +156,16 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void weigh_kernel(WeighParams P) {
     const int j1 = min(jn, first + min(block * BLOCK + BLOCK - 1, P.cols - 1) / P.gs + 1);   // (the last key of the block)
     if (j0 >= j1) continue;
     const int tiles = (j1 - j0 + WG_TILE - 1) / WG_TILE, subs = (j1 - j0 + 31) / 32;
+    // the first tile, the columns and what their sums were are requested together and waited for here, so that no wait for them
+    // stands between those for the tiles
+    stage(0);
+    uint4 q[KK];
+    f32x16_t off, inv;          // SUM: of the rows minus the reference, and the inverse sum
+    const int col = min(colw + (lane & 31), P.cols - 1), qi = col / P.gs;
+    const int low = first + min(colw, P.cols - 1) / P.gs, mine = first + qi;   // last keys of the tile's first and the lane's column
+    const uint16_t* const from = P.q + b * P.qb + qi * P.qt + (head * P.gs + col - qi * P.gs) * P.qh + 8 * (lane >> 5);
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) q[kk] = ri_ld16(from + 16 * kk);
     if (SUM) {   // the block's references and sums, joined from their splits where nobody has done so before
       if ((int)threadIdx.x < BLOCK) {
         const int col = block * BLOCK + threadIdx.x;
@@ -164,36 +174,18 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void weigh_kernel(WeighParams P) {
         sh_inv[SUM ? threadIdx.x : 0] = x.y;
       }
       __syncthreads();
-    }
-    uint4 q[KK];
-    f32x16_t off, inv;          // SUM: of the rows minus the reference, and the inverse sum
-    const int col = min(colw + (lane & 31), P.cols - 1), qi = col / P.gs;
-    const int low = first + min(colw, P.cols - 1) / P.gs, mine = first + qi;   // last keys of the tile's first and the lane's column
-    {
-      const uint16_t* from = P.q + b * P.qb + qi * P.qt + (head * P.gs + col - qi * P.gs) * P.qh + 8 * (lane >> 5);
 #pragma unroll
-      for (int kk = 0; kk < KK; ++kk) q[kk] = ri_ld16(from + 16 * kk);
-      if (SUM) {
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const float4 o = *reinterpret_cast<const float4*>(&sh_ref[wave * 32 + 8 * x + 4 * (lane >> 5)]);
-          const float4 f = *reinterpret_cast<const float4*>(&sh_inv[wave * 32 + 8 * x + 4 * (lane >> 5)]);
-          off[4 * x] = -o.x; off[4 * x + 1] = -o.y; off[4 * x + 2] = -o.z; off[4 * x + 3] = -o.w;
-          inv[4 * x] = f.x; inv[4 * x + 1] = f.y; inv[4 * x + 2] = f.z; inv[4 * x + 3] = f.w;
-        }
+      for (int x = 0; x < 4; ++x) {
+        const float4 o = *reinterpret_cast<const float4*>(&sh_ref[wave * 32 + 8 * x + 4 * (lane >> 5)]);
+        const float4 f = *reinterpret_cast<const float4*>(&sh_inv[wave * 32 + 8 * x + 4 * (lane >> 5)]);
+        off[4 * x] = -o.x; off[4 * x + 1] = -o.y; off[4 * x + 2] = -o.z; off[4 * x + 3] = -o.w;
+        inv[4 * x] = f.x; inv[4 * x + 1] = f.y; inv[4 * x + 2] = f.z; inv[4 * x + 3] = f.w;
       }
-      // waited for here, so that no wait for them stands between those for the tiles
+    }
 #pragma unroll
-      for (int kk = 0; kk < KK; ++kk) asm volatile("" : "+v"(q[kk].x), "+v"(q[kk].y), "+v"(q[kk].z), "+v"(q[kk].w));
-    }
+    for (int kk = 0; kk < KK; ++kk) asm volatile("" : "+v"(q[kk].x), "+v"(q[kk].y), "+v"(q[kk].z), "+v"(q[kk].w));
     weigh_wait<0>();
-    stage(0);
-    if (tiles > 1) {
-      stage(1);
-      weigh_wait<LOADS>();
-    } else {
-      weigh_wait<0>();
-    }
+    if (tiles > 1) stage(1);
     weigh_barrier();
     uint4 a[RING];
     const auto operand = [&](int buf, int sub, int kk) {

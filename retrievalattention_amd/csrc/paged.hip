@@ -4,6 +4,8 @@
 // pieces.  A table entry outside [0, pages) is a page that is not there: its rows are neither attended nor written.
 #include <math.h>
 
+#include <type_traits>
+
 #include "ri_common.h"
 
 #define PG_WAVES 8             // waves of an attending workgroup
@@ -72,7 +74,8 @@ __device__ __forceinline__ float pg_row_sum(float x) { return ri_xor_sum<1>(ri_x
 // share of `each`, whatever the lengths: places [i each, (i + 1) each).  A group that has rows begins with PG_LEAD places without
 // any, about what its query, its merge and its part cost (a workgroup with a dozen short groups was what all others waited for).
 // What workgroup i has of group g is part i + g: along the run either i or g moves on, so no two are the same.
-#define PG_SHARE 32   // places of a share at least
+#define PG_SHARE 8    // places of a share at least
+#define PG_WORKGROUPS 512   // that share the rows at most: parts of a group
 #define PG_LEAD 32
 // places of a group of sequence b
 __device__ __forceinline__ int pg_places(const PagedAttendParams& P, int b) {
@@ -100,7 +103,13 @@ __device__ __forceinline__ int pg_anew(int x) {
 __device__ __forceinline__ int64_t pg_uniform(int64_t x) {
   return (int64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)x) | (int64_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32;
 }
-// Whole workgroup: the run, and the sequence that has this workgroup's first place (nothing, where the run is shorter).
+// Workgroups that share so many places: as many as run at a time, two to a compute unit, where that leaves each four chunks to a wave;
+// below that one to a compute unit at most, of a chunk to a wave and more (one and a half to a unit, and some units have twice the others'
+// work: 8 groups of 16384 rows in 264 of them 23.8 us, in 256 19.2).
+__host__ __device__ __forceinline__ int pg_workgroups(int64_t places, int most) {
+  return places >= 32 * PG_WORKGROUPS || most < PG_WORKGROUPS / 2 ? most : PG_WORKGROUPS / 2;
+}
+// Whole workgroup: the run, and the sequence that has this workgroup's first place (B where the run is shorter).
 template <int THREADS>
 __device__ __forceinline__ PagedRun pg_run(const PagedAttendParams& P) {
   constexpr int NW = THREADS / 64;
@@ -111,6 +120,7 @@ __device__ __forceinline__ PagedRun pg_run(const PagedAttendParams& P) {
   const bool one = P.B <= THREADS;
   const int64_t heads = P.c.heads;
   int64_t sum = 0, each = 0;
+  if (threadIdx.x == 0) { sh_b = P.B; sh_from = 0; }
   for (int pass = one ? 1 : 0; pass < 2; ++pass) {   // the sum first; of few sequences everything at once
     int64_t in_front = 0;
     for (int b0 = 0; b0 < P.B; b0 += THREADS) {
@@ -128,7 +138,8 @@ __device__ __forceinline__ PagedRun pg_run(const PagedAttendParams& P) {
       }
       if (one) sum = all;
       if (pass) {
-        const int64_t share = (sum * heads + P.workgroups - 1) / P.workgroups;
+        const int workgroups = pg_workgroups(sum * heads, P.workgroups);
+        const int64_t share = (sum * heads + workgroups - 1) / workgroups;
         each = share < PG_SHARE ? PG_SHARE : share;
         const int64_t from = in_front + before, place = blockIdx.x * each;
         if (from * heads <= place && place < (from + n) * heads) {
@@ -170,8 +181,12 @@ __global__ __launch_bounds__(64 * PG_WAVES, UNI && GP < 16 ? 4 : 2) void paged_a
     if (at >= run.total) return;
     end = min(at + run.each, run.total);
     b = run.b;
-    const int mine = (int)(at - run.from * heads), per_head = pg_places(P, b);
+    if (b >= P.B) return;
+    // (Here and below, what is read a second time may have been written meanwhile, by a caller who did not wait for it: the result is
+    // undefined then, but no index leaves its buffer and every walk ends.)
+    const int mine = (int)(at - run.from * heads), per_head = max(pg_places(P, b), 1);
     head = mine / per_head;
+    if (head >= P.c.heads) return;
     skip = mine - head * per_head;
   }
 
@@ -194,6 +209,7 @@ __global__ __launch_bounds__(64 * PG_WAVES, UNI && GP < 16 ? 4 : 2) void paged_a
   int w0 = first & ~15, w1 = last;
   if (P.workgroups) {
     const int places = pg_places(P, b), mine = (int)min((int64_t)(places - skip), end - at);
+    if (mine <= 0) return;
     w1 = min(w0 + (max(skip + mine - PG_LEAD, 0) << 4), last);
     w0 += max(skip - PG_LEAD, 0) << 4;
     at += mine;
@@ -382,7 +398,10 @@ __global__ __launch_bounds__(64 * PG_WAVES, UNI && GP < 16 ? 4 : 2) void paged_a
   }
   if (at >= end) return;
   do {
-    if (++head == P.c.heads) { head = 0; ++b; }
+    if (++head == P.c.heads) {
+      head = 0;
+      if (++b == P.B) return;
+    }
   } while (pg_places(P, b) == 0);   // (there are places left, so there is such a group)
   skip = 0;
   __syncthreads();
@@ -391,13 +410,12 @@ __global__ __launch_bounds__(64 * PG_WAVES, UNI && GP < 16 ? 4 : 2) void paged_a
 
 #define PG_JOIN_THREADS 256
 #define PG_JOIN_ROWS (4 * PG_JOIN_THREADS)   // scores of a workgroup of the join
-#define PG_WORKGROUPS 1024                   // that share the rows at most: parts of a group
 
 // Grid (B * heads, (workgroups ? gs : 0) + ceil(max_len / PG_JOIN_ROWS) with scores): the first gs workgroups of a group join the
 // parts of a head each; the others add the weights of PG_JOIN_ROWS rows, exp(s - lse) summed over the heads, to the scores.
 template <int D, int GP, bool HALF>
 __global__ __launch_bounds__(PG_JOIN_THREADS) void paged_join_kernel(PagedAttendParams P) {
-  constexpr int NW = PG_JOIN_THREADS / 64, U = 8, DL = D / 64;   // DL: dims of a lane; U: parts requested at a time
+  constexpr int NW = PG_JOIN_THREADS / 64, DL = D / 64, MP = PG_WORKGROUPS / 64;   // DL: dims of a lane; MP: parts of a lane at most
   __shared__ float sh_M[16], sh_L[16], sh_f[PG_WORKGROUPS], sh_a[NW][D];
   const int g = blockIdx.x, b = g / P.c.heads, head = g - b * P.c.heads;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -409,20 +427,27 @@ __global__ __launch_bounds__(PG_JOIN_THREADS) void paged_join_kernel(PagedAttend
   if (!joins && (r0 >= last || r0 + PG_JOIN_ROWS <= first)) return;
   // the group's parts: of each workgroup that has rows of it
   const int2 share = P.workgroups && first < last ? P.shares[g] : make_int2(0, first < last ? 0 : -1);
-  const int parts = share.y - share.x + 1;
-  const size_t part0 = (size_t)g + share.x;
+  const int share0 = min(max(share.x, 0), max(P.workgroups - 1, 0)), parts = max(min(share.y, max(P.workgroups - 1, 0)) - share0 + 1, 0);
+  const size_t part0 = (size_t)g + share0;
   const float2* const ml = reinterpret_cast<const float2*>(P.part_ml) + part0 * GP;
   // maximum and sum of a head's parts, by a wave
   const auto join = [&](int j) {
     float M = -INFINITY, L = 0.f;
-    for (int s = lane; s < parts; s += 64) M = fmaxf(M, ml[(size_t)s * GP + j].x);
+    float2 x[MP];
+#pragma unroll
+    for (int i = 0; i < MP; ++i)
+      if (64 * i < parts) x[i] = ml[(size_t)min(64 * i + lane, parts - 1) * GP + j];
+#pragma unroll
+    for (int i = 0; i < MP; ++i)
+      if (64 * i < parts) M = fmaxf(M, x[i].x);
     M = ri_wave_max(M);
-    for (int s = lane; s < parts; s += 64) {
-      const float2 x = ml[(size_t)s * GP + j];
-      const float f = pg_weigh_part(x.x, x.y, M);
-      if (joins) sh_f[s] = f;
-      L += x.y * f;
-    }
+#pragma unroll
+    for (int i = 0; i < MP; ++i)
+      if (64 * i + lane < parts) {
+        const float f = pg_weigh_part(x[i].x, x[i].y, M);
+        if (joins) sh_f[64 * i + lane] = f;
+        L += x[i].y * f;
+      }
     L = ri_wave_sum(L);
     if (lane == 0) {
       sh_M[j] = M;
@@ -436,19 +461,24 @@ __global__ __launch_bounds__(PG_JOIN_THREADS) void paged_join_kernel(PagedAttend
     const float M = sh_M[j], L = sh_L[j];
     float A[DL] = {};
     const float* const acc = P.part_acc + (part0 * GP + j) * D + DL * lane;
-    for (int s = wave; s < parts; s += U * NW) {
-      float x[U][DL];
+    const auto add = [&](auto ahead) {   // so many parts are requested at a time
+      constexpr int U = decltype(ahead)::value;
+      for (int s = wave; s < parts; s += U * NW) {
+        float x[U][DL];
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+        for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int d = 0; d < DL; ++d) x[u][d] = acc[(size_t)min(s + u * NW, parts - 1) * GP * D + d];
+          for (int d = 0; d < DL; ++d) x[u][d] = acc[(size_t)min(s + u * NW, parts - 1) * GP * D + d];
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (s + u * NW < parts) {
+        for (int u = 0; u < U; ++u)
+          if (s + u * NW < parts) {
 #pragma unroll
-          for (int d = 0; d < DL; ++d) A[d] += x[u][d] * sh_f[s + u * NW];
-        }
-    }
+            for (int d = 0; d < DL; ++d) A[d] += x[u][d] * sh_f[s + u * NW];
+          }
+      }
+    };
+    if (parts > 8 * NW) add(std::integral_constant<int, 16>());
+    else add(std::integral_constant<int, 8>());
 #pragma unroll
     for (int d = 0; d < DL; ++d) sh_a[wave][DL * lane + d] = A[d];
     __syncthreads();
@@ -660,7 +690,7 @@ __device__ __forceinline__ int pg_pick(const int* hist, int bins, int& need) {
   }
   __syncthreads();
   need = sh_pick[1];
-  return sh_pick[0];
+  return sh_pick[0] & (bins - 1);
 }
 
 // Whole workgroup: exclusive sums over the threads of a count below 2^16 in each half of x; the workgroup's in *all.
@@ -700,9 +730,11 @@ __device__ __forceinline__ void pg_emit(const PagedFillParams& P, int g, int b, 
     const bool is_above = x.o[i] > lowest, is_tie = x.o[i] == lowest;
     if (is_above || (is_tie && tie < need)) {
       const int at = base + above + min(tie, need) - min(ties, need);
-      kept[at] = x.r0 + i;
-      if (scores) scores[at] = w[x.r0 + i];
-      if (positions) positions[at] = x.r0 + i;
+      if ((unsigned)at < (unsigned)P.budget) {   // (always, of lengths that stay as they are)
+        kept[at] = x.r0 + i;
+        if (scores) scores[at] = w[x.r0 + i];
+        if (positions) positions[at] = x.r0 + i;
+      }
     }
     above += is_above;
     tie += is_tie;
@@ -832,7 +864,7 @@ __device__ __forceinline__ uint32_t pg_lowest(const PagedFillParams& P, int g, i
     hist[threadIdx.x] = hist[threadIdx.x + PG_SEL_THREADS] = 0;
     __syncthreads();
     for (int c = wave; c < chunks; c += PG_SEL_WAVES) {
-      const int m = counts[c].y;
+      const int m = min(counts[c].y, PG_CHUNK);
       for (int i = lane; i < m; i += 64) {
         const uint32_t o = tied[(size_t)c * PG_CHUNK + i];
         if ((o & known) == lowest) atomicAdd(&hist[(o >> shift) & (bins - 1)], 1);
@@ -847,7 +879,7 @@ __device__ __forceinline__ uint32_t pg_lowest(const PagedFillParams& P, int g, i
 // By a wave: of a chunk's tied rows those above `lowest`, and in the upper half those of it.
 __device__ __forceinline__ uint32_t pg_kept_of(const uint32_t* tied, int m, uint32_t lowest) {
   uint32_t x = 0;
-  for (int i = threadIdx.x & 63; i < m; i += 64) {
+  for (int i = threadIdx.x & 63; i < min(m, PG_CHUNK); i += 64) {
     const uint32_t o = tied[i];
     x += (o > lowest ? 1u : 0u) + (o == lowest ? 0x10000u : 0u);
   }
@@ -936,7 +968,7 @@ __global__ __launch_bounds__(256) void paged_copy_kernel(PagedFillParams P) {
   if (row >= rows) return;
   const int src = n > P.budget ? P.kept[((size_t)b * P.c.heads + head) * P.budget + row] : row;
   const int page = P.c.table[b * P.c.ts + (row >> P.c.shift)], at = row & P.c.mask;
-  if ((unsigned)page >= (unsigned)P.c.pages) return;
+  if ((unsigned)page >= (unsigned)P.c.pages || (unsigned)src >= (unsigned)P.T) return;
   *reinterpret_cast<uint4*>(const_cast<uint16_t*>(P.c.k) + page * P.c.kp + head * P.c.kh + at * P.c.kr + piece) =
       ri_ld16(P.key + b * P.kb + src * P.kt + head * P.kh + piece);
   *reinterpret_cast<uint4*>(const_cast<uint16_t*>(P.c.v) + page * P.c.vp + head * P.c.vh + at * P.c.vr + piece) =
@@ -970,15 +1002,17 @@ static int paged_view(const ri_paged_t* c, int B, PagedView* v) {
 
 static int pg_pad(int gs) { return gs <= 4 ? 4 : gs <= 8 ? 8 : 16; }
 
-// Workgroups that share the rows: two to a compute unit, as many as run at a time, and twice as many from 128 groups on, of which
-// shares then are small parts (16 sequences of 1 .. 61440 tokens, 4 heads: 35 .. 95 us with 512, 41 .. 98 with 1024; 32 sequences of
-// 4096, 8 heads: 118 and 112).  None up to 512 rows: one to each group then, which leaves nothing to join (8 groups of 331 rows 8.2
-// us, shared 10 + 4).
+// Workgroups that share the rows of up to max_len.  None, one to each group, where that leaves no unit empty that a split would fill:
+// no shares to find, nothing to join, but the longest group sets the time, so up to 512 rows, and of many groups up to 2048.  Groups of four heads, us,
+// equal lengths | random ones | one long sequence among short ones; shared, then one to each group:
+//   8 x 513: 10.3; 8.6     8 x 1024: 10.2; 12.8     128 x 1024: 20.2 | 15.8 | 11.7; 16.1 | 15.0 | 12.9     256 x 2048: 55 | 34 | 18; 44 | 29 | 24
+//   512 x 2048: 100 | 61 | 20; 84 | 59 | 25     64 x 1024: 14.4 | 12.4 | 10.5; 15.4 | 14.3 | 12.9     256 x 4096: 93 | 57 | 20; 83 | 58 | 43
+// With scores the join is launched anyway, and the gain halves (256 x 1024 29.3 | 22.1 | 15.3; 28.3 | 21.0 | 17.0); the rule is the same,
+// so that an output does not depend on whether scores are asked for.
 static int paged_workgroups(int64_t groups, int max_len) {
-  if (max_len <= 512) return 0;
-  const int64_t shares = (groups * ((max_len + 15) / 16 + 1 + PG_LEAD) + PG_SHARE - 1) / PG_SHARE;
-  const int most = groups < 128 ? PG_WORKGROUPS / 2 : PG_WORKGROUPS;
-  return (int)(shares < most ? shares : most);
+  if (max_len <= 512 || (max_len <= 2048 && max_len <= groups * 6)) return 0;
+  const int64_t places = groups * ((max_len + 15) / 16 + 1 + PG_LEAD), shares = (places + PG_SHARE - 1) / PG_SHARE;
+  return pg_workgroups(places, shares < PG_WORKGROUPS ? (int)shares : PG_WORKGROUPS);
 }
 
 extern "C" size_t ri_paged_attention_workspace_bytes(int B, int heads, int gs, int dim, int max_len, int scored) {

@@ -89,6 +89,8 @@ CASES = [
     (HF, 5, 2, 1, 64, 8, [1, 1025, 2049, 513, 0], None),
     (BF, 1, 1, 2, 64, 32, [0], None),
     (BF, 70, 1, 4, 64, 16, [(37 * i) % 640 for i in range(70)], [(37 * i) % 640 // 2 for i in range(70)]),
+    # many groups: one workgroup to each
+    (HF, 170, 1, 4, 64, 16, [(37 * i) % 1000 for i in range(170)], None),
 ]
 
 

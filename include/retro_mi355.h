@@ -697,8 +697,9 @@ int ri_paged_attention(const ri_paged_t* cache, const void* q, const int32_t* le
  * sequence of n = lens[b] < budget rows takes them as row n.  Of a full one, with scores, they take the place of the row with the
  * lowest score in each head (equal scores: the lowest row; NaN counts as the highest), of those whose token is neither one of the
  * first `sinks` nor one of the last `recent`, the new one among them (if none is left, row 0); without scores nothing is written.
- * new_lens[b] = min(n + 1, budget) (another buffer than lens; may be NULL).  The row's score becomes 0 and its position, where
- * positions are given, token_positions[b], the token's place in the sequence.  sinks + recent < budget <= rows of the block table. */
+ * new_lens[b] = min(n + 1, budget) (in other memory than lens and token_positions; may be NULL).  The row's score becomes 0 and
+ * its position, where positions are given, token_positions[b], the token's place in the sequence.  sinks + recent < budget <= rows
+ * of the block table; keys and values lie in different pages. */
 int ri_paged_append(const ri_paged_t* cache, const void* key, const void* value, int64_t key_batch_stride,
                     int64_t key_head_stride, int64_t value_batch_stride, int64_t value_head_stride, const int32_t* lens,
                     int32_t* new_lens, float* scores, int64_t score_batch_stride, int64_t score_head_stride,
@@ -707,9 +708,10 @@ int ri_paged_append(const ri_paged_t* cache, const void* key, const void* value,
 
 /* Writes the prompts of B sequences, seqlens[b] (NULL: T) of T tokens each, into their pages from row 0 on.  Of a prompt of more
  * than `budget` tokens, each head keeps `budget`: the first `sinks`, the last `recent` and of the others those with the highest
- * weights[b, h, :] (order as above, equal weights: the first ones), in their order.  new_lens[b] = rows written (may be NULL);
- * scores and positions of the rows, where given, become the kept weights and the tokens' places.  weights may be NULL if T <=
- * budget and scores is.  sinks + recent <= budget. */
+ * weights[b, h, :] (order as above, equal weights: the first ones), in their order.  new_lens[b] = rows written (in other memory
+ * than seqlens; may be NULL); scores (in other memory than weights) and positions of the rows, where given, become the kept weights
+ * and the tokens' places.  weights may be NULL if T <= budget and scores is.  sinks + recent <= budget; keys and values lie in
+ * different pages. */
 size_t ri_paged_fill_workspace_bytes(int B, int heads, int T, int budget);
 int ri_paged_fill(const ri_paged_t* cache, const void* key, const void* value, int64_t key_batch_stride,
                   int64_t key_token_stride, int64_t key_head_stride, int64_t value_batch_stride, int64_t value_token_stride,

@@ -1102,7 +1102,9 @@ extern "C" int ri_paged_append(const ri_paged_t* cache, const void* key, const v
   P.token = token_positions;
   P.budget = budget; P.sinks = sinks; P.recent = recent; P.dim = cache->dim;
   const dim3 grid(cache->heads, B);
-  if (!scores || budget <= 2048) paged_append_kernel<256, 2><<<grid, 256, 0, (hipStream_t)stream>>>(P);
+  // (8 heads, 1024 rows 3.2 us, with 1024 threads 3.6; 4096 3.9 and 4.0; 8192 5.0 and 4.4; 32768 11.6 and 7.1; 256 heads, 4096 rows 4.1
+  // and 4.4, 8192 7.0 and 6.7: round trips and a launch, the rows' 8 bytes at most 4.7 TB/s)
+  if (!scores || budget <= 4096) paged_append_kernel<256, 2><<<grid, 256, 0, (hipStream_t)stream>>>(P);
   else paged_append_kernel<1024, 2><<<grid, 1024, 0, (hipStream_t)stream>>>(P);
   RI_HIP_CHECK_LAUNCH();
   return RI_OK;

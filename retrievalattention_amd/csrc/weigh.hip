@@ -371,7 +371,7 @@ static int weigh_up(int64_t n, int to) { return (int)((n + to - 1) / to * to); }
 // In the first one to a unit where two would have less than 1024 keys (one query, 32 heads, 8000 keys 16.5 us, with two 20.0; with more
 // keys two even out unequal lengths, 24 of up to 8340 keys, 516 columns 73 us, with one 78).
 // The second pass takes one block of columns to a workgroup, whose sums are a part of the result (8192 queries and keys, 32 heads:
-// parts of 67 MB), and more of them, which it adds up in LDS, where the parts would pass 256 MB.  Two blocks are one
+// parts of 67 MB; two blocks to each, added up in LDS, 381 us instead of 334), and more of them where the parts would pass 256 MB.  Two blocks are one
 // workgroup's of twice the waves (`wide`): they need not be added up by a launch of their own (256 columns, 8 heads: 2048 keys, 16
 // sequences 46.6 us, apart 50.0; 32768 keys 48 and 52; 131072 169 and 176).  Up to 32 splits are joined by whoever needs them, more by a
 // launch of their own (256 columns, 8 heads, 4096 keys: 16.4 us, with the launch 17.4; 64 splits of 8192 keys, four heads, 21.3 and 19.3).

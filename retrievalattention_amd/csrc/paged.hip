@@ -56,10 +56,25 @@ __device__ __forceinline__ f32x4_t pg_mfma32(uint4 a, uint4 b, f32x4_t c) {
   return HALF ? __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0)
               : __builtin_amdgcn_mfma_f32_16x16x32_bf16(ri_as_bf16x8(a), ri_as_bf16x8(b), c, 0, 0, 0);
 }
+
+// A probability p in [0, 1] as two elements, of which the first is below it and the second is what is left, rounded: their sum is within
+// 2^-16 of p (bfloat16) or 2^-22 (half) relative to it, where one element is within 2^-8 or 2^-11: with one, 6 to 30 % of the outputs
+// were not the exact result rounded, with two 0 to 0.3 % (fp32 throughout: 0 to 0.5 %).  It costs nothing: both parts fill one product of
+// 32 where one filled a product of 16 (four sequences of 131072 tokens 324 us either way).
+// Halves are of 2^15 p: their smallest normal number is 2^-14, and the weights of a long cache's rows are below it.  Both parts are
+// above 0 as long as an element holds them, so that an infinite value stays one.
 template <bool HALF>
-__device__ __forceinline__ f32x4_t pg_mfma16(pg_s4 a, pg_s4 b, f32x4_t c) {
-  return HALF ? __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4_t, a), __builtin_bit_cast(f16x4_t, b), c, 0, 0, 0)
-              : __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a, b, c, 0, 0, 0);
+__device__ __forceinline__ void pg_split(float p, uint16_t* first, uint16_t* left) {
+  const float x = HALF ? p * 32768.f : p;
+  const uint32_t below = max(__float_as_uint(x), 1u) - 1;   // (0 stays 0)
+  if (HALF) {
+    const auto h = __builtin_amdgcn_cvt_pkrtz(__uint_as_float(below), 0.f);
+    *first = __builtin_bit_cast(uint16_t, h[0]);
+    *left = ri_f32_to_e16<HALF>(x - (float)h[0]);
+  } else {
+    *first = (uint16_t)(below >> 16);
+    *left = ri_f32_to_e16<HALF>(x - __uint_as_float(below & 0xffff0000u));
+  }
 }
 
 // What a part's sums weigh relative to the maximum M of all.  A part without rows and one whose scores are all NaN have no maximum: its
@@ -168,7 +183,7 @@ __global__ __launch_bounds__(64 * PG_WAVES, UNI && GP < 16 ? 4 : 2) void paged_a
   constexpr int LPR = D / 8, RPI = 64 / LPR, NV = 16 / RPI;   // lanes to a value row, value rows to a load, loads to a chunk
   constexpr int TILE = (16 * VS * 2 > GP * D * 4) ? 16 * VS * 2 : GP * D * 4;
   __shared__ __attribute__((aligned(16))) char sh_tile[PG_WAVES][TILE];
-  __shared__ __attribute__((aligned(16))) uint16_t sh_p[PG_WAVES][16 * 16];
+  __shared__ __attribute__((aligned(16))) uint16_t sh_p[PG_WAVES][16 * 32];   // a head's: of rows 4 h .. the first parts, then what is left
   __shared__ __attribute__((aligned(16))) float sh_al[PG_WAVES][16];
   __shared__ float sh_m[PG_WAVES][GP], sh_l[PG_WAVES][GP];
 
@@ -194,7 +209,7 @@ __global__ __launch_bounds__(64 * PG_WAVES, UNI && GP < 16 ? 4 : 2) void paged_a
   uint16_t* const vt = (uint16_t*)sh_tile[wave];
   uint16_t* const pb = sh_p[wave];
   float* const al_sh = sh_al[wave];
-  reinterpret_cast<uint2*>(pb)[threadIdx.x & 63] = make_uint2(0u, 0u);
+  reinterpret_cast<uint4*>(pb)[threadIdx.x & 63] = ri_zero16();
   if ((threadIdx.x & 63) < 16) al_sh[threadIdx.x & 63] = 1.f;
   const int shift = P.c.shift, mask = P.c.mask;
   const int upc = UNI ? 1 : 16 >> shift;      // units, of which a lane holds the page, to a chunk
@@ -323,7 +338,8 @@ __global__ __launch_bounds__(64 * PG_WAVES, UNI && GP < 16 ? 4 : 2) void paged_a
       rescale |= al[i] != 1.f;
       l[i] = l[i] * al[i] + p;
       m[i] = mn;
-      pb[head_of(i) * 16 + n] = ri_f32_to_e16<HALF>(p);   // (half a step of a probability, for the matrix cores; sums are of p itself)
+      uint16_t* const to = pb + head_of(i) * 32 + (n >> 2) * 8 + (n & 3);   // (for the matrix cores; sums are of p itself)
+      pg_split<HALF>(p, to, to + 4);
     }
     const bool any = __builtin_amdgcn_ballot_w64(rescale) != 0;
     if (any && n == 0) {
@@ -338,13 +354,14 @@ __global__ __launch_bounds__(64 * PG_WAVES, UNI && GP < 16 ? 4 : 2) void paged_a
         acc[dt][0] *= a4.x; acc[dt][1] *= a4.y; acc[dt][2] *= a4.z; acc[dt][3] *= a4.w;
       }
     }
-    // lane (n, h): P of head n and rows 4 h .., V of those rows and dim 16 dt + n by transpose reads
-    const pg_s4 pa = *reinterpret_cast<const pg_s4*>(pb + n * 16 + 4 * h);
+    // lane (n, h): both parts of P of head n and rows 4 h .., and twice V of those rows and dim 16 dt + n by transpose reads
+    const uint4 pa = *reinterpret_cast<const uint4*>(pb + n * 32 + 8 * h);
     const uint16_t* vsrc = vt + (4 * h + (n >> 2)) * VS + 4 * (n & 3);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
       const pg_s4 vv = __builtin_amdgcn_ds_read_tr16_b64_v4i16((pg_s4 __attribute__((address_space(3)))*)(vsrc + 16 * dt));
-      acc[dt] = pg_mfma16<HALF>(pa, vv, acc[dt]);
+      const uint2 v2 = __builtin_bit_cast(uint2, vv);
+      acc[dt] = pg_mfma32<HALF>(pa, make_uint4(v2.x, v2.y, v2.x, v2.y), acc[dt]);
     }
     ri_wave_sync();
   }
@@ -365,7 +382,7 @@ __global__ __launch_bounds__(64 * PG_WAVES, UNI && GP < 16 ? 4 : 2) void paged_a
     const int hd = 4 * h2 + i;
     if (hd < GP) {
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) mine[hd * D + 16 * dt + n2] = acc[dt][i];
+      for (int dt = 0; dt < DT; ++dt) mine[hd * D + 16 * dt + n2] = HALF ? acc[dt][i] * 0x1p-15f : acc[dt][i];
     }
   }
   if (P.workgroups && tid == 0) {

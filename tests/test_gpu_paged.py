@@ -213,6 +213,73 @@ def test_attention_on_a_long_cache_past_32_bits(dev):
     assert torch.equal(k[32769, :, 700 - 512], key[0, 0])
 
 
+def _grid_scores(gen, dt, B, heads, gs, dim, page, rows, values):
+    """Queries of 1 in the first dimension and keys whose first element, of `values`, is the score: exact in either type."""
+    k, v, table = _pool(gen, dt, B, heads, dim, page, rows, junk=False)
+    k[..., 0] = values[torch.randint(len(values), k.shape[:3], generator=gen)].to(dt)
+    q = torch.zeros(B, 1, heads * gs, dim, dtype=dt)
+    q[..., 0] = 1
+    return q, k, v, table
+
+
+@pytest.mark.parametrize("dt,B,heads,gs,dim,page,lens", [
+    (BF, 2, 2, 4, 128, 16, [331, 64]),
+    (HF, 2, 2, 7, 128, 32, [300, 17]),
+    (BF, 1, 3, 16, 64, 8, [200]),
+    (HF, 1, 1, 3, 64, 4, [513]),
+    (BF, 2, 2, 4, 128, 16, [3001, 700]),
+])
+def test_attention_rounds_the_output_only(dev, dt, B, heads, gs, dim, page, lens):
+    """Values of 1 and -1 that nearly cancel: the weights' own error shows, not that of the result's last rounding."""
+    gen = torch.Generator().manual_seed(lens[0])
+    values = torch.arange(-64, 65) / 16        # scores of -4 .. 4
+    q, k, v, table = _grid_scores(gen, dt, B, heads, gs, dim, page, max(lens), values)
+    v = torch.where(torch.rand(v.shape, generator=gen) < 0.5, 1.0, -1.0).to(dt)
+    lens = torch.tensor(lens, dtype=torch.int32)
+    out = kernels.paged_attention(*(t.to(dev) for t in (q, k, v, table, lens)), scale=1.0)
+    want, _, _, absolute, size = oracle.attention(q, k, v, table, lens, None, 1.0)
+    # a weight's parts add up to it within 2^-16 (2^-21 in half); its score is rounded twice and its exponential twice, the sums in fp32
+    tol = _u(dt) * want.abs() + 2.0 ** (-16 if dt == BF else -21) * absolute + \
+        (8 * F * (1 + size[:, None, :, None]) + (64 + int(lens.max()) / 16) * F) * absolute
+    assert bool(((out.cpu().double() - want).abs() <= tol).all()), float(((out.cpu().double() - want).abs() / tol).max())
+
+
+@pytest.mark.parametrize("dt", [BF, HF], ids=["bf16", "f16"])
+@pytest.mark.parametrize("low", [9, 14, 18, 20])
+@pytest.mark.parametrize("n", [400, 5000])
+def test_attention_of_rows_that_weigh_little(dev, dt, low, n):
+    """One row takes nearly all the weight and has nothing to say; the result is the many others', of e^-low each."""
+    gen = torch.Generator().manual_seed(n + low)
+    heads, gs, dim, page = 2, 4, 64, 16
+    q, k, v, table = _grid_scores(gen, dt, 1, heads, gs, dim, page, n, torch.tensor([-float(low)]))
+    v = v.abs() + 1
+    k[int(table[0, 3]), :, 5, 0] = 0.0
+    v[int(table[0, 3]), :, 5] = 0.0
+    lens = torch.tensor([n], dtype=torch.int32)
+    out = kernels.paged_attention(*(t.to(dev) for t in (q, k, v, table, lens)), scale=1.0)
+    want, _, _, absolute, size = oracle.attention(q, k, v, table, lens, None, 1.0)
+    # as above; half: a part below its normal numbers is off by 2^-25 of 2^15 times a weight, and so is a result
+    tol = _u(dt) * want.abs() + 2.0 ** (-16 if dt == BF else -21) * absolute + (8 * F * (1 + low) + (64 + n / 16) * F) * absolute
+    if dt == HF:
+        tol = tol + n * 2.0 ** -40 * float(v.max()) + 2.0 ** -25
+    assert bool(((out.cpu().double() - want).abs() <= tol).all()), float(((out.cpu().double() - want).abs() / tol).max())
+
+
+@pytest.mark.parametrize("dt", [BF, HF], ids=["bf16", "f16"])
+def test_attention_of_infinite_values(dev, dt):
+    """A value of infinity that has weight is in the result, with the weight of the highest score as with others'."""
+    gen = torch.Generator().manual_seed(14)
+    heads, gs, dim, n = 1, 3, 64, 40
+    q, k, v, table = _grid_scores(gen, dt, 1, heads, gs, dim, 16, n, torch.tensor([-7.0, -3.5, -0.25]))
+    k[int(table[0, 1]), 0, 2, 0] = 0.0
+    v[int(table[0, 1]), 0, 2, 5] = math.inf
+    v[int(table[0, 2]), 0, 3, 9] = -math.inf
+    lens = torch.tensor([n], dtype=torch.int32)
+    out = kernels.paged_attention(*(t.to(dev) for t in (q, k, v, table, lens)), scale=1.0)
+    assert bool((out[..., 5] == math.inf).all()) and bool((out[..., 9] == -math.inf).all())
+    assert int(torch.isfinite(out).sum()) == heads * gs * (dim - 2)
+
+
 # ------------------------------------------------------------------------------------------------ append
 def _append_state(gen, dt, B, heads, dim, page, budget, lens, seen, sinks, recent, ties):
     k, v, table = _pool(gen, dt, B, heads, dim, page, budget, junk=False)

@@ -1065,8 +1065,9 @@ extern "C" int ri_paged_attention(const ri_paged_t* cache, const void* q, const 
   if (const int rc = paged_view(cache, B, &P.c)) return rc;
   if (!q || !lens || !out || !workspace || ri_any_misaligned16(q, out, workspace)) return RI_ERR_ARG;
   const int64_t groups = (int64_t)B * cache->heads;
-  if (gs <= 0 || gs > 16 || max_len <= 0 || max_len > cache->table_pages * cache->page_rows || groups > INT32_MAX / 16 || (int64_t)B * (max_len / 16 + 2 + PG_LEAD) > INT32_MAX)
-    return RI_ERR_ARG;   // (places of all sequences are counted in 32 bits)
+  if (gs <= 0 || gs > 16 || max_len <= 0 || max_len > cache->table_pages * cache->page_rows || groups > INT32_MAX / 16) return RI_ERR_ARG;
+  const int64_t places = max_len / 16 + 2 + PG_LEAD;   // of a group; those of a head's sequences and of a sequence's heads are counted in 32 bits
+  if (B * places > INT32_MAX || cache->heads * places > INT32_MAX) return RI_ERR_ARG;
   if (scores && (score_batch_stride < 0 || score_head_stride < max_len)) return RI_ERR_ARG;
   if (workspace_bytes < ri_paged_attention_workspace_bytes(B, cache->heads, gs, cache->dim, max_len, scores != nullptr))
     return RI_ERR_WORKSPACE;

@@ -438,7 +438,8 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     Py_RETURN_NONE;
   const int64_t hq = q->size(2), gs = hq / cache.heads, room = (int64_t)cache.table_pages * cache.page_rows;
   if (gs < 1 || gs > 16 || !paged_each(args[4], B, device, &lens, false) || !paged_each(args[5], B, device, &starts) ||
-      !paged_int(args[9], room, &max_len) || max_len < 1 || max_len > room || !paged_scale(args[7], cache.dim, &scale) ||
+      !paged_int(args[9], room, &max_len) || max_len < 1 || max_len > room ||
+      (max_len / 16 + 34) * (B > cache.heads ? B : cache.heads) > INT32_MAX || !paged_scale(args[7], cache.dim, &scale) ||
       !paged_values(args[6], at::kFloat, B, cache.heads, max_len, device, true, &scores, strides))
     Py_RETURN_NONE;
   const size_t bytes = ri_paged_attention_workspace_bytes((int)B, cache.heads, (int)gs, cache.dim, (int)max_len, scores != nullptr);

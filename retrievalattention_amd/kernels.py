@@ -933,6 +933,8 @@ def paged_attention(q, k_pages, v_pages, block_table, cache_seqlens, starts=None
     max_len = room if max_len is None else int(max_len)
     if not 1 <= max_len <= room:
         raise ValueError(f"max_len: expected 1 to {room}, the rows that the block table holds")
+    if (max_len // 16 + 34) * max(B, cache.heads) >= 1 << 31:
+        raise ValueError("max_len: too many rows for so many sequences or heads (16 of a sequence's heads are counted in 32 bits)")
     _table32(cache_seqlens, (B,), q.device, "cache_seqlens")
     if starts is not None:
         _table32(starts, (B,), q.device, "starts")

@@ -66,6 +66,14 @@ def test_attention(bad):
     assert _attention(**bad) == ARG
 
 
+@pytest.mark.parametrize("heads,B,answer", [(4096, 1, ARG), (2048, 1, ARG), (2047, 1, WORKSPACE), (65535, 1, ARG), (64, 2047, WORKSPACE),
+                                            (64, 2048, ARG)])
+def test_attention_of_more_rows_than_are_counted(heads, B, answer):
+    """Sixteen rows of a sequence's heads, or of all sequences' one head, are counted in 32 bits; a small workspace is refused behind that."""
+    big = _cache(heads=heads, table_pages=1 << 20)
+    assert _attention(big, B=B, max_len=1 << 24, bytes=16) == answer
+
+
 @pytest.mark.parametrize("scored", [0, 1])
 def test_attention_workspace(scored):
     need = lib().ri_paged_attention_workspace_bytes(3, 2, 4, 128, 64, scored)

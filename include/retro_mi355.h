@@ -723,7 +723,8 @@ int ri_paged_fill(const ri_paged_t* cache, const void* key, const void* value, i
 
 /* out[b, h, j] (fp32, [B, heads, T]) = sum over the gs query heads of head h and over the W queries of sequence b of the causal
  * attention weight that key j gets: query i is that of token seqlens[b] - W + i (seqlens NULL: T) and sees the keys up to its own;
- * queries of tokens before 0 weigh nothing, keys from seqlens[b] on get 0.  q [B, W, heads * gs, dim] and key [B, T, heads, dim]
+ * queries of tokens before 0 weigh nothing, keys from seqlens[b] on get 0; a query with a NaN among its scores makes the weights of the
+ * keys that it sees NaN, and no others.  q [B, W, heads * gs, dim] and key [B, T, heads, dim]
  * with strides in elements, multiples of 8; W <= T, gs <= 16, dim 64 or 128.  The workspace needs no initialisation. */
 size_t ri_attention_weights_workspace_bytes(int B, int heads, int gs, int W, int T);
 int ri_attention_weights(const void* q, const void* key, const int32_t* seqlens, float* out, int64_t q_batch_stride,

@@ -44,7 +44,7 @@ struct WeighParams {
 // A column's reference M and the inverse of its sum relative to M, of which a weight is exp(s - M) / sum, from its splits: this
 // thread takes `part`, part + of, ...; `of` neighbouring lanes together.  (Not the log-sum-exp alone: rounded to 32 bits it shifts all
 // weights of the column by up to half a unit of its size, 7e-7 of them, which is most of the error of a few queries' weights.)
-// A column without keys: inf and 0, so that a score less inf weighs 0.
+// A column without keys: inf and 0, so that a score less inf weighs 0.  One whose sum is NaN: inf and NaN.
 __device__ __forceinline__ float2 weigh_join(const WeighParams& P, int g, int col, int part, int of) {
   const float* const at = P.stats + ((size_t)g * P.S * P.cols_pad + col) * 2;
   float M = -INFINITY, L = 0.f;
@@ -60,7 +60,7 @@ __device__ __forceinline__ float2 weigh_join(const WeighParams& P, int g, int co
     L = L * __builtin_amdgcn_exp2f(M - ref) + l * __builtin_amdgcn_exp2f(m - ref);
     M = mn;
   }
-  return L != 0.f ? make_float2(M, 1.f / L) : make_float2(INFINITY, 0.f);
+  return L != L ? make_float2(INFINITY, L) : L != 0.f ? make_float2(M, 1.f / L) : make_float2(INFINITY, 0.f);
 }
 
 __device__ __forceinline__ int weigh_len(const WeighParams& P, int b) { return P.lens ? min(max(P.lens[b], 0), P.T) : P.T; }
@@ -118,6 +118,9 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void weigh_kernel(WeighParams P) {
   __shared__ __attribute__((aligned(16))) uint16_t sh[WG_BUFFERS][WG_TILE * D];
   __shared__ __attribute__((aligned(16))) float sh_ref[SUM ? BLOCK : 4], sh_inv[SUM ? BLOCK : 4];
   __shared__ float sh_part[SUM ? WG_BUFFERS : 1][SUM ? WAVES : 1][WG_TILE];
+  // The last key that a column with a NaN for its sum sees.  The weights up to that key are made NaN at the end; the column's own
+  // share is made 0, since the keys that it does not see have a share of every column, too.
+  __shared__ int sh_nan_key;
   extern __shared__ float sh_sum[];   // [rows], with several blocks
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = blockIdx.x, b = g / P.heads, head = g - b * P.heads;
@@ -149,7 +152,9 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void weigh_kernel(WeighParams P) {
   float* const to = !SUM ? nullptr : P.supers > 1 ? P.part + ((size_t)g * P.supers + super) * P.T : P.out + (size_t)g * P.T;
   if (SUM && P.per > 1)
     for (int i = threadIdx.x; i < P.rows; i += 64 * WAVES) sh_sum[i] = 0.f;
+  if (SUM && threadIdx.x == 0) sh_nan_key = -1;
   float m = -INFINITY, l = 0.f;
+  int nan_key = -1;   // (of the column that this thread looks up)
 
   for (int block = block0; block < block1; ++block) {
     const int colw = block * BLOCK + wave * 32;
@@ -171,7 +176,8 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void weigh_kernel(WeighParams P) {
         const int col = block * BLOCK + threadIdx.x;
         const float2 x = P.joined ? P.norms[(size_t)g * P.cols_pad + col] : weigh_join(P, g, col, 0, 1);
         sh_ref[SUM ? threadIdx.x : 0] = x.x;
-        sh_inv[SUM ? threadIdx.x : 0] = x.y;
+        sh_inv[SUM ? threadIdx.x : 0] = x.y != x.y ? 0.f : x.y;
+        if (x.y != x.y) nan_key = first + col / P.gs;   // (columns, and their keys, ascend)
       }
       __syncthreads();
 #pragma unroll
@@ -311,10 +317,12 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void weigh_kernel(WeighParams P) {
   }
 
   if (SUM) {
+    if (nan_key >= 0) atomicMax(&sh_nan_key, nan_key);
     __syncthreads();
     // nobody reads what a part has of keys behind the last that its columns see; in the result those weigh nothing
     const int seen = max(min(jn, weigh_last_key(P, n, super, BLOCK) + 1) - j0, 0), all = P.supers > 1 ? seen : min(P.rows, P.T - j0);
     for (int i = (P.per > 1 ? 0 : seen) + threadIdx.x; i < all; i += 64 * WAVES) to[j0 + i] = i < seen ? sh_sum[i] : 0.f;
+    for (int i = threadIdx.x; i < min(sh_nan_key + 1, jn) - j0; i += 64 * WAVES) to[j0 + i] = NAN;   // (below `seen`)
     return;
   }
   const float M = ri_xor_max<32>(m);

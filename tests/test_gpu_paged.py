@@ -505,6 +505,46 @@ def test_prompt_weights_of_equal_keys(dev, T, dim):
     assert bool(((got * T - 1).abs() <= 2 * F).all())
 
 
+@pytest.mark.parametrize("bad", [math.nan, math.inf], ids=["nan", "inf"])
+@pytest.mark.parametrize("where", [0.0, 0.4, 1.0], ids=["first", "middle", "last"])
+@pytest.mark.parametrize("dt,T,W,heads,gs,dim,n", [
+    (BF, 70, 9, 2, 4, 128, 70),
+    (HF, 70, 40, 1, 3, 64, 33),
+    (BF, 700, 300, 2, 2, 64, 640),
+    (BF, 500, 500, 1, 4, 128, 500),
+    (HF, 900, 70, 1, 3, 128, 901 - 13),
+])
+def test_prompt_weights_of_a_spoilt_query(dev, dt, T, W, heads, gs, dim, n, where, bad):
+    """The keys that it sees have a NaN, those behind its token the other queries' weights, other heads what they had."""
+    gen = torch.Generator().manual_seed(T + W + gs)
+    q, key = _randn(gen, 2, W, heads * gs, dim).to(dt), _randn(gen, 2, T, heads, dim).to(dt)
+    lens = torch.tensor([n, T], dtype=torch.int32)
+    scale = dim ** -0.5
+    clean, size = oracle.weigh(q, key, lens, scale)
+    was = kernels.attention_weights(q.to(dev), key.to(dev), seqlens=lens.to(dev)).cpu()
+    i, j = max(W - n, int(where * (W - 1))), gs - 1      # a query that is one of the prompt's; a head of the first key-value head
+    last = n - W + i
+    p = torch.softmax(key[0, :last + 1, 0].double() @ q[0, i, j].double() * scale, 0)
+    clean[0, 0, :last + 1] -= p
+    q[0, i, j, 5] = bad
+    got = kernels.attention_weights(q.to(dev), key.to(dev), seqlens=lens.to(dev)).cpu()
+    assert bool(got[0, 0, :last + 1].isnan().all())
+    rel = 4 * (dim + 12) * F * (1 + size) + (64 + T / 32 + W * gs / 32) * F     # (as in test_prompt_weights)
+    assert bool(((got[0, 0, last + 1:].double() - clean[0, 0, last + 1:]).abs() <= rel[0, 0] * clean[0, 0, last + 1:] + 1e-30).all())
+    assert torch.equal(got[1], was[1]) and torch.equal(got[0, 1:], was[0, 1:])
+
+
+@pytest.mark.parametrize("T,W,at", [(70, 9, 0), (300, 300, 299), (900, 20, 450)])
+def test_prompt_weights_of_a_spoilt_key(dev, T, W, at):
+    """Every query behind it sees it, so nothing of its head is known: the last token's query sees all."""
+    gen = torch.Generator().manual_seed(T)
+    q, key = _randn(gen, 1, W, 4, 64).to(BF), _randn(gen, 1, T, 2, 64).to(BF)
+    was = kernels.attention_weights(q.to(dev), key.to(dev))
+    key[0, at, 1, 9] = math.nan
+    got = kernels.attention_weights(q.to(dev), key.to(dev))
+    assert bool(got[0, 1].isnan().all()) and torch.equal(got[0, 0], was[0, 0])
+
+
 def test_prompt_weights_far_apart(dev):
     """Scores that rise along the prompt by more than an exponential of fp32 can tell, and fall."""
     gen = torch.Generator().manual_seed(10)

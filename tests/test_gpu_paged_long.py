@@ -1,0 +1,81 @@
+"""The paged cache's operators where a workgroup has much to do: many tiles of a prompt's weights.  Which
+sizes those are is the launches' rule; tests/test_paged_plans.py asks it whether the cases here are still what they are meant to be.
+Compared with 64 bits on the device; u = eps / 2 of the element type and F = 2^-24 count roundings."""
+import math
+
+import pytest
+import torch
+
+from retrievalattention_amd import kernels
+
+pytestmark = pytest.mark.gpu
+
+BF, HF = torch.bfloat16, torch.float16
+F = 2.0 ** -24
+
+# dt, heads, gs, dim, W, T, lens
+ENDS = [20011, 19000 - 31, 16500, 321, 300, 250, 190, 130, 97, 5, 0]   # inside a split, of 1 to 6 tiles and odd halves of one, and nothing
+STREAMED = [
+    (BF, 4, 1, 128, 5, 20011, ENDS),          # a part of one block of columns
+    (HF, 4, 4, 64, 16, 20011, ENDS),
+    (BF, 4, 4, 128, 64, 20011, ENDS),         # two blocks in one workgroup
+    (HF, 3, 7, 64, 33, 20011, ENDS),
+    (BF, 2, 4, 64, 200, 20011, ENDS),         # several blocks
+    (HF, 2, 5, 128, 100, 20011, ENDS),
+    (BF, 1, 3, 128, 9000, 9000, [9000, 8199, 4097, 500]),   # whole prompts
+    (HF, 2, 4, 128, 64, 90001, [90001, 61002]),             # splits that a launch of its own joins
+]
+
+
+def _randn(gen, dev, *shape):
+    return torch.randn(*shape, generator=gen, device=dev)
+
+
+def _weigh(q, key, n, scale):
+    """Weights [n] that the queries [W, gs, dim] of the last W tokens give the first n keys [T, dim], and the largest sum of |q k| scale."""
+    W, gs, dim = q.shape
+    out, size = torch.zeros(n, dtype=torch.float64, device=q.device), 0.0
+    k, w = key[:n].double().T.contiguous(), min(W, n)
+    step = max(1, (1 << 24) // max(n, 1))
+    for i0 in range(W - w, W, step):
+        i1 = min(i0 + step, W)
+        last = n - W + torch.arange(i0, i1, device=q.device)
+        later = torch.arange(n, device=q.device)[None] > last[:, None]
+        for j in range(gs):
+            x = (q[i0:i1, j].double() @ k).mul_(scale)
+            out += torch.softmax(x.masked_fill_(later, -math.inf), 1).sum(0)
+            size = max(size, float((q[i0:i1, j].abs().float() @ k.abs().float()).max()) * scale * 1.0001)
+    return out, size
+
+
+def _check_weights(got, q, key, lens, gs, pairs):
+    dim, W, T = q.shape[3], q.shape[1], key.shape[1]
+    for b, h in pairs:
+        n = lens[b]
+        want, size = _weigh(q[b, :, h * gs:(h + 1) * gs], key[b, :, h], n, dim ** -0.5)
+        # an exponential's argument is a sum of dim products in fp32, up to `size`, less one of that order; sums of T terms for a query
+        # and of W * gs terms for a key
+        rel = 4 * (dim + 12) * F * (1 + size) + (64 + T / 32 + W * gs / 32) * F
+        d = (got[b, h, :n].double() - want).abs()
+        assert bool((d <= rel * want + 1e-30).all()), (b, h, float((d / want.clamp(min=1e-30)).max()), rel)
+        assert bool((got[b, h, n:] == 0).all()), (b, h)
+
+
+def _prompts(dev, dt, heads, gs, dim, W, T, lens):
+    gen = torch.Generator(device=dev).manual_seed(T + W + gs)
+    B = len(lens)
+    key = _randn(gen, dev, B, T, heads, dim).to(dt)
+    q = _randn(gen, dev, B, W, heads * gs, dim).to(dt)
+    for b, n in enumerate(lens):   # what lies behind a prompt's end has no say
+        key[b, n:] = math.nan
+        q[b, :max(0, W - n)] = math.nan
+    return q, key, torch.tensor(lens, dtype=torch.int32, device=dev)
+
+
+@pytest.mark.parametrize("dt,heads,gs,dim,W,T,lens", STREAMED)
+def test_prompt_weights_of_many_tiles(dev, dt, heads, gs, dim, W, T, lens):
+    q, key, lens_t = _prompts(dev, dt, heads, gs, dim, W, T, lens)
+    got = kernels.attention_weights(q, key, seqlens=lens_t)
+    _check_weights(got, q, key, lens, gs, [(b, h) for b in range(len(lens)) for h in range(heads)])
+    for _ in range(5):
+        assert torch.equal(kernels.attention_weights(q, key, seqlens=lens_t), got)

@@ -1,0 +1,72 @@
+"""What the rules of the paged cache's launches (csrc/weigh_plan.h, host code: compiled here by g++) make of the
+cases that the GPU tests were written for: a rule that changes must not take a test off the code that it is about."""
+import ctypes
+import os
+import shutil
+import subprocess
+
+import pytest
+
+from tests import test_gpu_paged_long as cases
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def _compiled(tmp_path_factory, header, function):
+    if shutil.which("g++") is None:
+        pytest.skip("no g++")
+    where = tmp_path_factory.mktemp("plan")
+    (where / "plan.cpp").write_text(f'#include "{header}"\nextern "C" {function}\n')
+    subprocess.run(["g++", "-std=c++17", "-O1", "-shared", "-fPIC", "-I", os.path.join(ROOT, "retrievalattention_amd", "csrc"),
+                    str(where / "plan.cpp"), "-o", str(where / "plan.so")], check=True)
+    return ctypes.CDLL(str(where / "plan.so")).ask
+
+
+class Weigh(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int) for n in ("cols_pad", "S", "rows", "S2", "rows2", "per", "supers")] + [("joined", ctypes.c_bool),
+                                                                                                       ("wide", ctypes.c_bool)]
+
+
+@pytest.fixture(scope="module")
+def weigh_plan(tmp_path_factory):
+    call = _compiled(tmp_path_factory, "weigh_plan.h",
+                     "void ask(long long groups, int cols, int T, WeighPlan* p) { *p = weigh_plan(groups, cols, T); }")
+
+    def plan(groups, cols, T):
+        p = Weigh()
+        call(ctypes.c_longlong(groups), cols, T, ctypes.byref(p))
+        return p
+    return plan
+
+
+def _walks(plan, second, cols, gs, W, T, lens):
+    """(tiles of 64 keys, halves of a tile) of every workgroup's walk over a block of columns."""
+    rows, block = (plan.rows2, 256 if plan.wide else 128) if second else (plan.rows, 256)
+    walks = set()
+    for n in lens:
+        for c in range(0, cols, block):
+            end = min(n, n - W + min(c + block - 1, cols - 1) // gs + 1)
+            for j0 in range(0, T, rows):
+                keys = min(j0 + rows, end) - j0
+                if keys > 0:
+                    walks.add((-(-keys // 64), -(-keys // 32)))
+    return walks
+
+
+def test_prompt_weights_stream_many_tiles(weigh_plan):
+    """Both passes, of eight waves and of four, of 64 and 128 dims and either way of joining: walks of 1 to 6 tiles and of more, that end
+    in either half of a tile."""
+    walks, joined, supers = {}, set(), set()
+    for _, heads, gs, dim, W, T, lens in cases.STREAMED:
+        plan = weigh_plan(len(lens) * heads, W * gs, T)
+        assert plan.per == 1 and plan.rows >= 7 * 64 and plan.rows2 >= 7 * 64
+        joined.add(plan.joined)
+        supers.add(min(plan.supers, 16))
+        for key in ((dim, "first"), (dim, "wide" if plan.wide else "second")):
+            walks.setdefault(key, set()).update(_walks(plan, key[1] != "first", W * gs, gs, W, T, lens))
+    assert {1, 16} < supers and min(supers - {1}) < 16 and joined == {False, True}
+    assert len(walks) == 6
+    for key, seen in walks.items():
+        tiles = {t for t, _ in seen}
+        assert {1, 2, 3, 4, 5, 6} <= tiles and max(tiles) > 6, (key, sorted(tiles))
+        assert {s % 2 for t, s in seen if t > 1} == {0, 1}, key

@@ -1,4 +1,4 @@
-"""The paged cache's operators where a workgroup has much to do: many tiles of a prompt's weights.  Which
+"""The paged cache's operators where a workgroup has much to do: many tiles and several column blocks of a prompt's weights.  Which
 sizes those are is the launches' rule; tests/test_paged_plans.py asks it whether the cases here are still what they are meant to be.
 Compared with 64 bits on the device; u = eps / 2 of the element type and F = 2^-24 count roundings."""
 import math
@@ -24,6 +24,12 @@ STREAMED = [
     (HF, 2, 5, 128, 100, 20011, ENDS),
     (BF, 1, 3, 128, 9000, 9000, [9000, 8199, 4097, 500]),   # whole prompts
     (HF, 2, 4, 128, 64, 90001, [90001, 61002]),             # splits that a launch of its own joins
+]
+# the same, and the (sequence, head) pairs that are compared: several blocks to a workgroup
+BLOCKS = [
+    (BF, 8, 16, 128, 1011, 8300, [8300, 8300, 4111, 1500, 700, 64, 1, 0], [(0, 0), (1, 7), (2, 3), (3, 0), (4, 6), (5, 1), (6, 2), (7, 4)]),
+    (HF, 4, 16, 64, 8192, 24000, [24000, 23333], [(0, 1), (1, 3)]),
+    (BF, 8, 4, 128, 17000, 17000, [17000], [(0, 0), (0, 7)]),
 ]
 
 
@@ -79,3 +85,21 @@ def test_prompt_weights_of_many_tiles(dev, dt, heads, gs, dim, W, T, lens):
     _check_weights(got, q, key, lens, gs, [(b, h) for b in range(len(lens)) for h in range(heads)])
     for _ in range(5):
         assert torch.equal(kernels.attention_weights(q, key, seqlens=lens_t), got)
+
+
+@pytest.mark.parametrize("dt,heads,gs,dim,W,T,lens,pairs", BLOCKS)
+def test_prompt_weights_of_several_blocks_to_a_workgroup(dev, dt, heads, gs, dim, W, T, lens, pairs):
+    """Sums of several blocks of columns are added up in LDS where the parts of one each would be too many."""
+    q, key, lens_t = _prompts(dev, dt, heads, gs, dim, W, T, lens)
+    got = kernels.attention_weights(q, key, seqlens=lens_t)
+    _check_weights(got, q, key, lens, gs, pairs)
+    assert torch.equal(kernels.attention_weights(q, key, seqlens=lens_t), got)
+    (b, h), n = pairs[0], lens[pairs[0][0]]
+    for i in (W - min(W, n), W // 2, W - 1):    # a query with a NaN: what it sees, and only that
+        bad = q.clone()
+        bad[b, i, h * gs + gs // 2, 1] = math.nan
+        spoilt = kernels.attention_weights(bad, key, seqlens=lens_t)
+        last = n - W + i
+        assert bool(spoilt[b, h, :last + 1].isnan().all()) and bool(spoilt[b, h, last + 1:].isfinite().all())
+        spoilt[b, h] = got[b, h]
+        assert torch.equal(spoilt, got)

@@ -70,3 +70,14 @@ def test_prompt_weights_stream_many_tiles(weigh_plan):
         tiles = {t for t, _ in seen}
         assert {1, 2, 3, 4, 5, 6} <= tiles and max(tiles) > 6, (key, sorted(tiles))
         assert {s % 2 for t, s in seen if t > 1} == {0, 1}, key
+
+
+def test_prompt_weights_give_a_workgroup_several_blocks(weigh_plan):
+    """Two and three, with fewer left for the last one, and blocks that begin in front of the prompt or see none of a split."""
+    plans = {}
+    for _, heads, gs, dim, W, T, lens, _ in cases.BLOCKS:
+        plan = weigh_plan(len(lens) * heads, W * gs, T)
+        blocks = -(-W * gs // 128)
+        assert plan.per > 1 and plan.supers > 1 and plan.supers == -(-blocks // plan.per)
+        plans[plan.per] = (blocks % plan.per != 0) or plans.get(plan.per, False)
+    assert plans == {2: True, 3: True}

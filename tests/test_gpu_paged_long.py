@@ -1,4 +1,5 @@
-"""The paged cache's operators where a workgroup has much to do: many tiles and several column blocks of a prompt's weights.  Which
+"""The paged cache's operators where a workgroup has much to do: pages past a wave's first 64 table entries,
+many tiles and several column blocks of a prompt's weights.  Which
 sizes those are is the launches' rule; tests/test_paged_plans.py asks it whether the cases here are still what they are meant to be.
 Compared with 64 bits on the device; u = eps / 2 of the element type and F = 2^-24 count roundings."""
 import math
@@ -31,6 +32,13 @@ BLOCKS = [
     (HF, 4, 16, 64, 8192, 24000, [24000, 23333], [(0, 1), (1, 3)]),
     (BF, 8, 4, 128, 17000, 17000, [17000], [(0, 0), (0, 7)]),
 ]
+
+# dt, heads, gs, dim, page, lens, starts: long caches of few pages that repeat, whose rows many workgroups share
+LONG = [(dt, 8, gs, 64, page, [180000 - 997 * b for b in range(8)], [0, 16, 40017, 5, 0, 1023, 77777, 64])
+        for dt, gs, page in ((BF, 4, 1), (HF, 1, 2), (BF, 8, 4), (HF, 3, 8), (BF, 4, 16), (HF, 12, 64), (HF, 5, 16), (BF, 16, 8))]
+LONG += [(BF, 2, 4, 128, 64, [1500000, 0, 1400001, 3000000], [7, 0, 1, 500003]),
+         (HF, 2, 7, 128, 16, [2500000, 2600000], None),
+         (BF, 4, 16, 128, 4, [600000, 900001], [0, 31])]
 
 
 def _randn(gen, dev, *shape):
@@ -103,3 +111,66 @@ def test_prompt_weights_of_several_blocks_to_a_workgroup(dev, dt, heads, gs, dim
         assert bool(spoilt[b, h, :last + 1].isnan().all()) and bool(spoilt[b, h, last + 1:].isfinite().all())
         spoilt[b, h] = got[b, h]
         assert torch.equal(spoilt, got)
+
+
+def _attend(q, k_pages, v_pages, table, n, start, scale):
+    """One sequence and head: q [gs, dim], pages [pages, page_rows, dim], table [n]; out, lse, weights, sums of p |v|, largest sum of |q k| scale."""
+    page = k_pages.shape[1]
+    k, v = k_pages.reshape(-1, k_pages.shape[2]).double(), v_pages.reshape(-1, v_pages.shape[2]).double()
+    r = torch.arange(start, n, device=q.device)
+    at = table.long()[r // page] * page + r % page
+    x = (q.double() @ k.T.contiguous() * scale)[:, at]
+    size = (q.double().abs() @ k.abs().T.contiguous() * scale).max(1).values
+    p = torch.softmax(x, 1)
+    # rows repeat: their weights first
+    each = torch.zeros(q.shape[0], k.shape[0], dtype=torch.float64, device=q.device).index_add_(1, at, p)
+    return each @ v, torch.logsumexp(x, 1), p, each @ v.abs(), size
+
+
+def _check_attention(dev, dt, heads, gs, dim, page, lens, starts, pool=64):
+    gen = torch.Generator(device=dev).manual_seed(lens[0] + page + gs)
+    B, per = len(lens), -(-max(lens) // page)
+    pool = max(pool, 2048 // page)
+    k, v = _randn(gen, dev, pool, heads, page, dim).to(dt), _randn(gen, dev, pool, heads, page, dim).to(dt)
+    table = torch.randint(pool, (B, per), generator=gen, device=dev, dtype=torch.int32)
+    q = (2 * _randn(gen, dev, B, 1, heads * gs, dim)).to(dt)
+    lens_t = torch.tensor(lens, dtype=torch.int32, device=dev)
+    starts_t = None if starts is None else torch.tensor(starts, dtype=torch.int32, device=dev)
+    before = torch.rand(B, heads, max(lens), generator=gen, device=dev)
+    scores = before.clone()
+    out, lse = kernels.paged_attention(q, k, v, table, lens_t, starts=starts_t, scores=scores, max_len=max(lens), return_softmax_lse=True)
+    plain = kernels.paged_attention(q, k, v, table, lens_t, starts=starts_t, max_len=max(lens))
+    assert torch.equal(plain, out)
+    u = torch.finfo(dt).eps / 2
+    for b in range(B):
+        first = min(starts[b] if starts else 0, lens[b])
+        for h in range(heads):
+            mine = slice(h * gs, (h + 1) * gs)
+            got, got_lse, after = out[b, 0, mine].double(), lse[b, mine].double(), scores[b, h]
+            untouched = torch.ones(max(lens), dtype=torch.bool, device=dev)
+            untouched[first:lens[b]] = False
+            assert torch.equal(after[untouched], before[b, h][untouched])
+            if first == lens[b]:
+                assert bool((got == 0).all()) and bool((got_lse == -math.inf).all())
+                continue
+            want, want_lse, p, absolute, size = _attend(q[b, 0, mine], k[:, h], v[:, h], table[b], lens[b], first, dim ** -0.5)
+            # a score is a sum of dim products in fp32, scaled (two roundings more); its exponential is off by that and by two units.
+            # A weight's two parts add up to it within 2^-16 (2^-21 in half, and 2^-40 of what the highest score weighs); a result
+            # below the normal halves is off by 2^-25.
+            n = lens[b] - first
+            ds = (dim + 4) * F * size + 8 * F * (1 + size)
+            tol = u * want.abs() + (2.0 ** (-16 if dt == BF else -21) + 2 * ds[:, None] + (64 + n / 16) * F) * absolute
+            if dt == HF:
+                tol = tol + n * 2.0 ** -40 * p.max(1).values[:, None] * v[:, h].abs().max().double() + 2.0 ** -25
+            assert bool(((got - want).abs() <= tol).all()), (b, h, float(((got - want).abs() / tol).max()))
+            assert bool(((got_lse - want_lse).abs() <= ds + (64 + n / 16) * F + 4 * F * want_lse.abs()).all()), (b, h)
+            w = p.sum(0)
+            want_scores = before[b, h, first:lens[b]].double() + w
+            rel = 2 * ds.max() + (64 + n / 16) * F
+            assert bool(((after[first:lens[b]].double() - want_scores).abs() <= rel * w + 18 * F * want_scores).all()), (b, h)
+
+
+@pytest.mark.parametrize("dt,heads,gs,dim,page,lens,starts", LONG)
+def test_attention_past_a_waves_first_table_entries(dev, dt, heads, gs, dim, page, lens, starts):
+    """A wave holds 64 entries of the table at a time, the next 64 behind them: every row's weight and the output tell which were used."""
+    _check_attention(dev, dt, heads, gs, dim, page, lens, starts)

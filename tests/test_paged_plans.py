@@ -1,4 +1,4 @@
-"""What the rules of the paged cache's launches (csrc/weigh_plan.h, host code: compiled here by g++) make of the
+"""What the rules of the paged cache's launches (csrc/paged_plan.h, csrc/weigh_plan.h: compiled here by g++) make of the
 cases that the GPU tests were written for: a rule that changes must not take a test off the code that it is about."""
 import ctypes
 import os
@@ -81,3 +81,42 @@ def test_prompt_weights_give_a_workgroup_several_blocks(weigh_plan):
         assert plan.per > 1 and plan.supers > 1 and plan.supers == -(-blocks // plan.per)
         plans[plan.per] = (blocks % plan.per != 0) or plans.get(plan.per, False)
     assert plans == {2: True, 3: True}
+
+
+@pytest.fixture(scope="module")
+def shares(tmp_path_factory):
+    """The workgroups that share a call's rows, and each one's place in the run: (workgroups, [(sequence, head, chunks)] of each)."""
+    call = _compiled(tmp_path_factory, "paged_plan.h", """long long ask(long long groups, int max_len, long long total, int* workgroups) {
+        *workgroups = paged_workgroups(groups, max_len); return *workgroups ? pg_each(total, *workgroups) : 0; }""")
+    call.restype = ctypes.c_longlong
+
+    def walk(heads, lens, starts=None, max_len=None):
+        first = [min(s, n) for s, n in zip(starts or [0] * len(lens), lens)]
+        chunks = [-(-n // 16) - s // 16 if s < n else 0 for s, n in zip(first, lens)]
+        places = [c + 32 if c else 0 for c in chunks]      # (a group begins with 32 places without rows)
+        total, workgroups = sum(places) * heads, ctypes.c_int()
+        each = call(ctypes.c_longlong(heads * len(lens)), max_len or max(lens), ctypes.c_longlong(total), ctypes.byref(workgroups))
+        if not workgroups.value:
+            return 0, []
+        runs, at = [[] for _ in range(workgroups.value)], 0
+        for b, n in enumerate(places):
+            for h in range(heads if n else 0):
+                for i in range(at // each, -(-(at + n) // each)):
+                    rows = min(at + n, (i + 1) * each) - max(at + 32, i * each)
+                    if rows > 0:
+                        runs[i].append((b, h, rows))
+                at += n
+        return workgroups.value, runs
+    return walk
+
+
+def test_attention_walks_past_the_first_table_entries(shares):
+    """Waves that look at three and more batches of 64 table entries, with pages of every size, beginning in the middle too."""
+    seen = {}
+    for _, heads, gs, dim, page, lens, starts in cases.LONG:
+        workgroups, runs = shares(heads, lens, starts)
+        to_batch = 64 // (1 if page >= 16 else 16 // page)
+        most = max(-(-chunks // 8) for run in runs for _, _, chunks in run)      # of a wave, eight to a workgroup
+        assert workgroups == 512 and -(-most // to_batch) >= 3, (page, most)
+        seen.setdefault(min(page, 16), set()).add(1 if gs <= 4 else 2 if gs <= 8 else 4)
+    assert set(seen) == {1, 2, 4, 8, 16} and set().union(*seen.values()) == {1, 2, 4}

@@ -1,6 +1,6 @@
-"""The paged cache's operators where a workgroup has much to do: pages past a wave's first 64 table entries,
-many tiles and several column blocks of a prompt's weights.  Which
-sizes those are is the launches' rule; tests/test_paged_plans.py asks it whether the cases here are still what they are meant to be.
+"""The paged cache's operators where there is much to do: pages past a wave's first 64 table entries, groups of many parts,
+more sequences than threads, many tiles and several column blocks of a prompt's weights.  Which sizes those are is the launches' rule;
+tests/test_paged_plans.py asks it whether the cases here are still what they are meant to be.
 Compared with 64 bits on the device; u = eps / 2 of the element type and F = 2^-24 count roundings."""
 import math
 
@@ -39,6 +39,11 @@ LONG = [(dt, 8, gs, 64, page, [180000 - 997 * b for b in range(8)], [0, 16, 4001
 LONG += [(BF, 2, 4, 128, 64, [1500000, 0, 1400001, 3000000], [7, 0, 1, 500003]),
          (HF, 2, 7, 128, 16, [2500000, 2600000], None),
          (BF, 4, 16, 128, 4, [600000, 900001], [0, 31])]
+# the same: many parts to a group, which the join's waves take 64 at a time
+PARTS = [(BF, 1, 4, 128, 64, [131072], None), (HF, 1, 7, 64, 16, [70001, 0, 41000], [3, 0, 999]), (BF, 2, 16, 64, 16, [300001], [70]),
+         (HF, 1, 16, 128, 32, [600000], None), (BF, 1, 1, 64, 8, [16000, 270000, 17, 0, 33], [15999, 0, 0, 0, 32])]
+# sequences beyond the 512 that a workgroup looks at at a time, sharing their rows: dt, heads, gs, dim, page, room, sequences
+MANY = [(BF, 1, 4, 64, 16, 2304, 700), (HF, 2, 1, 64, 64, 2560, 1300), (BF, 1, 3, 128, 8, 3000, 513), (HF, 1, 8, 64, 32, 5000, 1025)]
 
 
 def _randn(gen, dev, *shape):
@@ -174,3 +179,25 @@ def _check_attention(dev, dt, heads, gs, dim, page, lens, starts, pool=64):
 def test_attention_past_a_waves_first_table_entries(dev, dt, heads, gs, dim, page, lens, starts):
     """A wave holds 64 entries of the table at a time, the next 64 behind them: every row's weight and the output tell which were used."""
     _check_attention(dev, dt, heads, gs, dim, page, lens, starts)
+
+
+@pytest.mark.parametrize("dt,heads,gs,dim,page,lens,starts", PARTS)
+def test_attention_of_many_parts(dev, dt, heads, gs, dim, page, lens, starts):
+    _check_attention(dev, dt, heads, gs, dim, page, lens, starts)
+
+
+def _many_lengths(room, B):
+    """Most empty or short, long ones first, last, and on both sides of each 512th."""
+    gen = torch.Generator().manual_seed(B)
+    lens = (torch.rand(B, generator=gen) ** 6 * room).int()
+    lens[torch.rand(B, generator=gen) < 0.5] = 0
+    for b in (0, 1, 510, 511, 512, 513, 1023, 1024, B - 2, B - 1):
+        if b < B:
+            lens[b] = room - 7 * (b % 13)
+    return lens.tolist()
+
+
+@pytest.mark.parametrize("dt,heads,gs,dim,page,room,B", MANY)
+def test_attention_shares_the_rows_of_many_sequences(dev, dt, heads, gs, dim, page, room, B):
+    lens = _many_lengths(room, B)
+    _check_attention(dev, dt, heads, gs, dim, page, lens, [n // 3 if b % 2 else 0 for b, n in enumerate(lens)])

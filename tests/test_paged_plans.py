@@ -120,3 +120,27 @@ def test_attention_walks_past_the_first_table_entries(shares):
         assert workgroups == 512 and -(-most // to_batch) >= 3, (page, most)
         seen.setdefault(min(page, 16), set()).add(1 if gs <= 4 else 2 if gs <= 8 else 4)
     assert set(seen) == {1, 2, 4, 8, 16} and set().union(*seen.values()) == {1, 2, 4}
+
+
+def test_attention_joins_many_parts(shares):
+    """More than 64 to a group, up to all 512 that there are, and groups whose parts begin at a later workgroup."""
+    most, later = [], False
+    for _, heads, gs, dim, page, lens, starts in cases.PARTS:
+        _, runs = shares(heads, lens, starts)
+        of = {}
+        for i, run in enumerate(runs):
+            for b, h, _ in run:
+                of.setdefault((b, h), []).append(i)
+        most.append(max(len(p) for p in of.values()))
+        later |= any(len(p) > 64 and p[0] > 0 for p in of.values())
+    assert min(most) > 64 and max(most) > 448 and later and len({-(-m // 64) for m in most}) >= 3, most
+
+
+def test_attention_shares_the_rows_of_more_sequences_than_threads(shares):
+    for _, heads, gs, dim, page, room, B in cases.MANY:
+        lens = cases._many_lengths(room, B)
+        workgroups, runs = shares(heads, lens, [n // 3 if b % 2 else 0 for b, n in enumerate(lens)])
+        assert B > 512 and workgroups > 0
+        assert any(run and run[0][0] > 511 for run in runs) and any(run and run[0][0] < 512 for run in runs)
+        if B > 1024:
+            assert any(run and run[0][0] > 1023 for run in runs)

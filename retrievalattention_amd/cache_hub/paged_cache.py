@@ -93,14 +93,29 @@ class paged_cache:
             raise RuntimeError(f"paged_cache: a sequence has {self.rows} rows, all that it was built for")
         self._take({b: min(n + 1, self.rows) for b, n in enumerate(self._rows) if self._table[b]})
 
+    def _rows_of(self, t, batch, tokens, heads, name):
+        """Refuses what the kernels would refuse of a layer's rows [batch, tokens, heads, head_dim] before pages are handed out for them."""
+        kernels._strided(t, 4, self.dtype, self.block_table.device, name)
+        if t.shape != (batch, tokens, heads, self.head_dim):
+            raise ValueError(f"{name}: expected [{batch}, {tokens}, {heads}, {self.head_dim}]")
+
     # ------------------------------------------------------------------ prompt
     def prefill_update_kv_cache(self, query_states, key_states, value_states, layer_idx, batch_idx):
         """One sequence's prompt in one layer: query [1, T, heads, dim] (only read with a budget), key and value [1, T, kv heads,
         dim].  Returns key and value as they came, for the prompt's own attention."""
+        if not isinstance(key_states, torch.Tensor) or key_states.dim() != 4:
+            raise ValueError("paged_cache: expected key [1, T, kv heads, head_dim]")
         T, b = key_states.shape[1], batch_idx
         if not 0 <= b < self.batch_size or T < 1 or key_states.shape[0] != 1:
             raise ValueError(f"paged_cache: expected a prompt [1, 1 token or more, ..] and a place below {self.batch_size}")
         if layer_idx == 0:
+            self._rows_of(key_states, 1, T, self.kv_head, "key_states")
+            self._rows_of(value_states, 1, T, self.kv_head, "value_states")
+            if self.budget is not None:
+                heads = query_states.shape[2] if isinstance(query_states, torch.Tensor) and query_states.dim() == 4 else 0
+                if heads % self.kv_head or not 1 <= heads // self.kv_head <= kernels.MAX_GROUP_SIZE:
+                    raise ValueError(f"query_states: expected 1 to {kernels.MAX_GROUP_SIZE} heads to each key-value head")
+                self._rows_of(query_states, 1, T, heads, "query_states")
             if self.budget is None and T > self.rows:
                 raise ValueError(f"paged_cache: a prompt of {T} tokens, built for {self.rows}")
             wanted = -(-min(T, self.rows) // self.page_size)
@@ -131,6 +146,8 @@ class paged_cache:
     def decode_update_kv_cache(self, key_states, value_states, layer_idx):
         """The next token's key and value [B, 1, kv heads, dim] in one layer."""
         if layer_idx == 0 and not torch.cuda.is_current_stream_capturing():
+            self._rows_of(key_states, self.batch_size, 1, self.kv_head, "key_states")
+            self._rows_of(value_states, self.batch_size, 1, self.kv_head, "value_states")
             self.prepare_token()
         kernels.paged_append(key_states, value_states, self.k_pages[layer_idx], self.v_pages[layer_idx], self.block_table,
                              self.seqlens, self.new_seqlens, **self._per_row(layer_idx),

@@ -89,3 +89,41 @@ def test_refusals():
                 dict(budget=10, sinks=0, recent=0), dict(window=0)):
         with pytest.raises(ValueError):
             _cache(**bad)
+
+
+def _state(c):
+    return ([list(row) for row in c._table], list(c._rows), sorted(c._free), c.block_table.tolist(), c.seqlens.tolist(), c.seen.tolist(),
+            c.active.tolist())
+
+
+@pytest.mark.parametrize("budget", [None, 24])
+def test_refused_tensors_change_nothing(budget, monkeypatch):
+    """A prompt or a token of other shapes, types or layouts than the pages' is refused before a sequence ends or pages are taken."""
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    c = _cache(**({} if budget is None else dict(budget=budget, sinks=2, recent=4)))
+    _prompt(c, 0, 16)
+    _prompt(c, 2, 20)
+    before = _state(c)
+    key, token = torch.zeros(1, 30, 1, 64, dtype=torch.bfloat16), torch.zeros(3, 1, 1, 64, dtype=torch.bfloat16)
+    query = torch.zeros(1, 30, 2, 64, dtype=torch.bfloat16)
+    bad = [key.half(), key.float(), key[..., :32], torch.zeros(1, 30, 2, 64, dtype=torch.bfloat16), key[0], None, "key",
+           torch.zeros(1, 30, 1, 128, dtype=torch.bfloat16)[..., ::2]]
+    for x in bad:
+        for k, v in ((x, key), (key, x)):
+            with pytest.raises((ValueError, TypeError)):
+                c.prefill_update_kv_cache(query, k, v, 0, 0)
+            assert _state(c) == before
+    with pytest.raises((ValueError, TypeError)):
+        c.prefill_update_kv_cache(query, key, key[:, :29], 0, 0)
+    if budget is not None:
+        for x in (None, query.half(), query[:, :29], query[0], query[0, 0], torch.zeros(1, 30, 17, 64, dtype=torch.bfloat16)):
+            with pytest.raises((ValueError, TypeError)):
+                c.prefill_update_kv_cache(x, key, key, 0, 0)
+    assert _state(c) == before
+    for x in (token.half(), token[:2], token[..., :32], token[:, 0], None, torch.zeros(3, 2, 1, 64, dtype=torch.bfloat16)):
+        for k, v in ((x, token), (token, x)):
+            with pytest.raises((ValueError, TypeError)):
+                c.decode_update_kv_cache(k, v, 0)
+            assert _state(c) == before
+    c.prefill_update_kv_cache(query, key, key, 0, 0)
+    assert c._rows[0] == (30 if budget is None else 24)

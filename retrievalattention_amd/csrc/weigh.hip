@@ -115,9 +115,9 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void weigh_kernel(WeighParams P) {
   __shared__ __attribute__((aligned(16))) uint16_t sh[WG_BUFFERS][WG_TILE * D];
   __shared__ __attribute__((aligned(16))) float sh_ref[SUM ? BLOCK : 4], sh_inv[SUM ? BLOCK : 4];
   __shared__ float sh_part[SUM ? WG_BUFFERS : 1][SUM ? WAVES : 1][WG_TILE];
-  // The last key that a column with a NaN for its sum sees.  The weights up to that key are made NaN at the end; the column's own
-  // share is made 0, since the keys that it does not see have a share of every column, too.
-  __shared__ int sh_nan_key;
+  // The last key that a column with a NaN for its sum sees, of the columns that a wave looks up.  The weights up to that key are made NaN
+  // at the end; the column's own share is made 0, since the keys that it does not see have a share of every column, too.
+  __shared__ int sh_nan[SUM ? WAVES / 2 : 1];
   extern __shared__ float sh_sum[];   // [rows], with several blocks
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = blockIdx.x, b = g / P.heads, head = g - b * P.heads;
@@ -149,9 +149,8 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void weigh_kernel(WeighParams P) {
   float* const to = !SUM ? nullptr : P.supers > 1 ? P.part + ((size_t)g * P.supers + super) * P.T : P.out + (size_t)g * P.T;
   if (SUM && P.per > 1)
     for (int i = threadIdx.x; i < P.rows; i += 64 * WAVES) sh_sum[i] = 0.f;
-  if (SUM && threadIdx.x == 0) sh_nan_key = -1;
+  if (SUM && wave < WAVES / 2) sh_nan[SUM ? wave : 0] = -1;   // (a wave's own until the barrier behind its columns)
   float m = -INFINITY, l = 0.f;
-  int nan_key = -1;   // (of the column that this thread looks up)
 
   for (int block = block0; block < block1; ++block) {
     const int colw = block * BLOCK + wave * 32;
@@ -174,7 +173,7 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void weigh_kernel(WeighParams P) {
         const float2 x = P.joined ? P.norms[(size_t)g * P.cols_pad + col] : weigh_join(P, g, col, 0, 1);
         sh_ref[SUM ? threadIdx.x : 0] = x.x;
         sh_inv[SUM ? threadIdx.x : 0] = x.y != x.y ? 0.f : x.y;
-        if (x.y != x.y) nan_key = first + col / P.gs;   // (columns, and their keys, ascend)
+        if (x.y != x.y) atomicMax(&sh_nan[SUM ? wave : 0], first + col / P.gs);
       }
       __syncthreads();
 #pragma unroll
@@ -314,12 +313,16 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void weigh_kernel(WeighParams P) {
   }
 
   if (SUM) {
-    if (nan_key >= 0) atomicMax(&sh_nan_key, nan_key);
-    __syncthreads();
-    // nobody reads what a part has of keys behind the last that its columns see; in the result those weigh nothing
+    // (Where the part's columns see some of these keys a block was done, and a barrier stood behind it.)
+    // Nobody reads what a part has of keys behind the last that its columns see; in the result those weigh nothing.
     const int seen = max(min(jn, weigh_last_key(P, n, super, BLOCK) + 1) - j0, 0), all = P.supers > 1 ? seen : min(P.rows, P.T - j0);
     for (int i = (P.per > 1 ? 0 : seen) + threadIdx.x; i < all; i += 64 * WAVES) to[j0 + i] = i < seen ? sh_sum[i] : 0.f;
-    for (int i = threadIdx.x; i < min(sh_nan_key + 1, jn) - j0; i += 64 * WAVES) to[j0 + i] = NAN;   // (below `seen`)
+    if (seen > 0) {
+      int nan_key = -1;
+#pragma unroll
+      for (int w = 0; w < WAVES / 2; ++w) nan_key = max(nan_key, sh_nan[SUM ? w : 0]);
+      for (int i = threadIdx.x; i < min(nan_key + 1, jn) - j0; i += 64 * WAVES) to[j0 + i] = NAN;
+    }
     return;
   }
   const float M = ri_xor_max<32>(m);

@@ -684,8 +684,9 @@ typedef struct ri_paged_t {
 
 /* Attention of one token of each of B sequences over its rows [starts[b], lens[b]) (starts NULL: from 0 on; both clamped to
  * [0, max_len], max_len at most the rows of the block table, and max_len / 16 + 34 times B or the heads below 2^31):
- * out[b, i, :] = sum_r p_r v_r with p = softmax(scale q[b, i, :].k_r), q and out [B, heads * gs, dim] contiguous, gs <= 16; lse_out [B, heads * gs] fp32 (or NULL) the log of the sum of the
- * exponentials.  No rows: zeros and -inf.  With scores, the weights p_r summed over the gs heads of head h are added to
+ * out[b, i, :] = sum_r p_r v_r with p = softmax(scale q[b, i, :].k_r), q and out [B, heads * gs, dim] contiguous, gs <= 16;
+ * lse_out [B, heads * gs] fp32 (or NULL) the log of the sum of the exponentials.  No rows, or none whose score is above -inf: zeros
+ * and -inf.  With scores, the weights p_r summed over the gs heads of head h are added to
  * scores[b * score_batch_stride + h * score_head_stride + r] (fp32, score_head_stride >= max_len).  The workspace needs no
  * initialisation; calls that may overlap must not share it. */
 size_t ri_paged_attention_workspace_bytes(int B, int heads, int gs, int dim, int max_len, int scored);

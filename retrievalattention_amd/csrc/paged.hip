@@ -59,8 +59,9 @@ __device__ __forceinline__ f32x4_t pg_mfma32(uint4 a, uint4 b, f32x4_t c) {
 
 // A probability p in [0, 1] as two elements, of which the first is below it and the second is what is left, rounded: their sum is within
 // 2^-16 of p (bfloat16) or 2^-22 (half) relative to it, where one element is within 2^-8 or 2^-11: with one, 6 to 30 % of the outputs
-// were not the exact result rounded, with two 0 to 0.3 % (fp32 throughout: 0 to 0.5 %).  It costs nothing: both parts fill one product of
-// 32 where one filled a product of 16 (four sequences of 131072 tokens 324 us either way).
+// were not the exact result rounded, with two 0 to 0.3 % (fp32 throughout: 0 to 0.5 %).  It costs 0 to 2 %, since both parts fill
+// one product of 32 where one filled a product of 16 (us, one part and two: four sequences of 131072 tokens, 8 heads of 4, 324 and 324; 32
+// of 4096 with scores 98.7 and 98.9; one of 331 7.7 and 7.8; 256 of 400, 8 heads of 16, 88.7 and 90.4).
 // Halves are of 2^15 p: their smallest normal number is 2^-14, and the weights of a long cache's rows are below it.  Both parts are
 // above 0 as long as an element holds them, so that an infinite value stays one.
 template <bool HALF>
@@ -161,7 +162,8 @@ __device__ __forceinline__ PagedRun pg_run(const PagedAttendParams& P) {
 // lane / 16) gets the scores of cache row n for the heads 4 h + i of A's rows, of which it keeps GP / 4, so that every (row, head) is
 // some lane's once.
 // UNI: a chunk lies in one page (pages of 16 rows and more), whose address is the same for the whole wave.  Four waves to a SIMD where
-// that spills nothing: four sequences of 16384 tokens in pages of 8 rows 59 us with two, 66 with four, in pages of 16 51 with four.
+// that spills nothing: four sequences of 16384 tokens in pages of 8 rows 51 us with two, 57 with four, in pages of 16 50 and 47; 64 of 500
+// 25.8 and 23.3.
 template <int D, int GP, bool HALF, bool UNI>
 __global__ __launch_bounds__(64 * PG_WAVES, UNI && GP < 16 ? 4 : 2) void paged_attend_kernel(PagedAttendParams P) {
   constexpr int NH = GP / 4, DT = D / 16, KK = D / 32, VS = D + 16;

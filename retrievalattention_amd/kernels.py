@@ -913,8 +913,8 @@ def paged_attention(q, k_pages, v_pages, block_table, cache_seqlens, starts=None
     table that is no page of the pool stands for rows that are not there.  starts [B] int32: the first row that is attended.
     scores [B, heads, rows] fp32: each row's weights, summed over the gs query heads of its head, are added to it.
     max_len: no sequence has more rows (default: what the table holds; rows from max_len on are not attended), which sizes the
-    split over workgroups and the workspace.  Returns out like q, zeros where no row is attended, and with return_softmax_lse the
-    log-sum-exp [B, heads * gs] (-inf there).  `scratch`: the caller's own Scratch, where calls may overlap others."""
+    split over workgroups and the workspace.  Returns out like q, zeros where no row is attended or none has a score
+    above -inf, and with return_softmax_lse the log-sum-exp [B, heads * gs] (-inf there).  `scratch`: the caller's own Scratch, where calls may overlap others."""
     out = step_calls().paged_attention(q, k_pages, v_pages, block_table, cache_seqlens, starts, scores, scale, return_softmax_lse,
                                        max_len, _held(q, "paged", scratch))
     if out is not None:
@@ -1040,7 +1040,7 @@ def attention_weights(q, key, seqlens=None, scale=None, scratch=None):
     """The causal attention weights that the last W tokens of each prompt give its keys, summed over them and over the gs query
     heads of a key-value head: fp32 [B, heads, T], 0 past a prompt's end.  q [B, W, heads * gs, dim], the queries of the last W
     tokens (of all: W = T); key [B, T, heads, dim]; seqlens [B] int32: the prompts' lengths (default T), query i being that of token
-    seqlens[b] - W + i (one before token 0 weighs nothing)."""
+    seqlens[b] - W + i (one before token 0 weighs nothing).  A NaN among a query's scores makes the weights of the keys that it sees NaN."""
     out = step_calls().attention_weights(q, key, seqlens, scale, _held(key, "weights", scratch))
     if out is not None:
         return check(out, "attention_weights") if out.__class__ is int else out

@@ -280,6 +280,32 @@ def test_attention_of_infinite_values(dev, dt):
     assert int(torch.isfinite(out).sum()) == heads * gs * (dim - 2)
 
 
+@pytest.mark.parametrize("n", [40, 700, 5000])
+def test_attention_of_scores_of_minus_infinity(dev, n):
+    """A head all of whose scores are -inf attends nothing; one of which some are attends the others."""
+    gen = torch.Generator().manual_seed(n)
+    heads, gs, dim = 2, 3, 64
+    q, k, v, table = _grid_scores(gen, BF, 1, heads, gs, dim, 16, n, torch.arange(-32, 33) / 16)
+    rows = torch.arange(n)
+    p = table[0].long()[rows // 16]
+    k[p, 0, rows % 16, 0] = -math.inf
+    some = rows[torch.rand(n, generator=gen) < 0.5]
+    k[table[0].long()[some // 16], 1, some % 16, 0] = -math.inf
+    lens = torch.tensor([n], dtype=torch.int32)
+    before = torch.rand(1, heads, table.shape[1] * 16, generator=gen)
+    scores = before.to(dev)
+    out, lse = kernels.paged_attention(*(t.to(dev) for t in (q, k, v, table, lens)), scale=1.0, scores=scores, return_softmax_lse=True)
+    assert bool((out[0, 0, :gs] == 0).all()) and bool((lse[0, :gs] == -math.inf).all()) and torch.equal(scores[0, 0].cpu(), before[0, 0])
+    x = k[p, 1, rows % 16, 0].double()
+    w = torch.softmax(x, 0)
+    want = w @ v[p, 1, rows % 16].double()
+    tol = _u(BF) * want.abs() + (2.0 ** -16 + (24 + 64 + n / 16) * F) * (w @ v[p, 1, rows % 16].double().abs())   # (scores of up to 2)
+    assert bool(((out[0, 0, gs:].cpu().double() - want).abs() <= tol).all())
+    got = scores[0, 1, :n].cpu().double()
+    assert bool(((got - before[0, 1, :n].double() - gs * w).abs() <= (24 + 64 + n / 16) * F * gs * w + 18 * F * got).all())
+    assert torch.equal(got.float()[w == 0], before[0, 1, :n][w == 0])
+
+
 # ------------------------------------------------------------------------------------------------ append
 def _append_state(gen, dt, B, heads, dim, page, budget, lens, seen, sinks, recent, ties):
     k, v, table = _pool(gen, dt, B, heads, dim, page, budget, junk=False)

@@ -509,10 +509,12 @@ __global__ __launch_bounds__(PG_JOIN_THREADS) void paged_join_kernel(PagedAttend
   }
   for (int j = wave; j < P.gs; j += NW) join(j);
   __syncthreads();
+  bool spoilt = false;
 #pragma unroll
   for (int j = 0; j < GP; ++j) {
     const float M = sh_M[min(j, P.gs - 1)], L = sh_L[min(j, P.gs - 1)];
     if (j >= P.gs || L == 0.f) continue;   // (no rows: nothing to add)
+    spoilt |= L != L;
     const float inv = 1.f / L;
 #pragma unroll
     for (int i = 0; i < 4; ++i) was[i] += pg_exp2(x[i].x[j] - M) * inv;
@@ -520,7 +522,12 @@ __global__ __launch_bounds__(PG_JOIN_THREADS) void paged_join_kernel(PagedAttend
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int r = r0 + threadIdx.x + PG_JOIN_THREADS * i;
-    if (r >= first && r < last) scores[r] = was[i];
+    if (r < first || r >= last) continue;
+    if (spoilt) {   // the weights are NaN, and not those of rows that are not there
+      const int page = P.c.table[b * P.c.ts + (r >> P.c.shift)];
+      if ((unsigned)page >= (unsigned)P.c.pages) continue;
+    }
+    scores[r] = was[i];
   }
 }
 

@@ -306,6 +306,29 @@ def test_attention_of_scores_of_minus_infinity(dev, n):
     assert torch.equal(got.float()[w == 0], before[0, 1, :n][w == 0])
 
 
+@pytest.mark.parametrize("page,n", [(16, 300), (8, 700), (64, 3000)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf], ids=["nan", "inf"])
+def test_attention_leaves_scores_of_rows_that_are_not_there(dev, page, n, bad):
+    """Also where a NaN makes the others' scores NaN, and with another head's weights as they are."""
+    gen = torch.Generator().manual_seed(n)
+    heads, gs, dim = 2, 3, 64
+    k, v, table = _pool(gen, BF, 1, heads, dim, page, n)
+    table[0, 1], table[0, n // page // 2] = -1, k.shape[0]
+    q = (2 * _randn(gen, 1, 1, heads * gs, dim)).to(BF)
+    lens = torch.tensor([n], dtype=torch.int32)
+    before = torch.rand(1, heads, table.shape[1] * page, generator=gen)
+    on = lambda t: t.to(dev)  # noqa: E731
+    clean, spoilt = on(before), on(before)
+    kernels.paged_attention(on(q), on(k), on(v), on(table), on(lens), scores=clean)
+    q[0, 0, 1, 3] = bad
+    kernels.paged_attention(on(q), on(k), on(v), on(table), on(lens), scores=spoilt)
+    rows = torch.arange(before.shape[2])
+    there = (rows < n) & (table[0].long()[rows // page] >= 0) & (table[0].long()[rows // page] < k.shape[0])
+    for got in (clean.cpu(), spoilt.cpu()):
+        assert torch.equal(got[:, :, ~there], before[:, :, ~there])
+    assert bool(spoilt[0, 0].cpu()[there].isnan().all()) and torch.equal(spoilt[0, 1], clean[0, 1])
+
+
 # ------------------------------------------------------------------------------------------------ append
 def _append_state(gen, dt, B, heads, dim, page, budget, lens, seen, sinks, recent, ties):
     k, v, table = _pool(gen, dt, B, heads, dim, page, budget, junk=False)
